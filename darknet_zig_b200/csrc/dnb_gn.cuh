@@ -1,0 +1,193 @@
+// Group norm on channels-last tensors: how the work is cut, shared by the forward (dnb_gn.cu) and the
+// backward (dnb_gn_bwd.cu).
+//
+// A unit is one image's run of whole groups, `cb` channels wide (64 bytes of a row or more, so that the
+// accesses of a row fill their sectors) and all `spatial` rows tall. A CTA, or a cluster of up to 8 CTAs
+// that split the rows, loads a unit into shared memory once, forms the statistics there and writes the
+// outputs from there, so every tensor crosses HBM once. Units beyond what 8 CTAs can hold take the
+// streaming path: partial statistics of row chunks, a merge, and a second read of the inputs.
+//
+// A thread owns one vector of channels (VB bytes) and every RL-th row, so per-channel values sit in its
+// registers: V = cb / N vectors make a row; RL = T / V threads share a column, or, where a row is longer
+// than the block, the block walks the columns in passes of T vectors.
+#pragma once
+
+#include <atomic>
+
+#include "dnb_types.cuh"
+
+namespace dnb {
+
+struct GnPlan {
+    int vb = 16;            // bytes of a vector
+    int64_t cb = 0;         // channels of a unit (the last unit of an image may have fewer)
+    int64_t nu = 0;         // units of an image
+    int cluster = 1;        // CTAs of a unit
+    int64_t rows = 0;       // rows of a CTA
+    int threads = 256;
+    bool stream = false;
+    int64_t chunks = 1;     // row chunks of a unit on the streaming path
+    size_t slab = 0;        // bytes of one tensor's rows in shared memory, rounded to 16
+    size_t part_floats = 0; // floats of one per-thread partial array
+    size_t smem = 0;
+};
+
+constexpr size_t kGnSmemTarget = 100 * 1024;  // two CTAs an SM
+constexpr size_t kGnSmemMax = 200 * 1024;
+constexpr size_t kGnStreamSlab = 32 * 1024;   // a streaming chunk's rows
+constexpr int kGnMaxCluster = 8;
+constexpr int64_t kGnMaxGroup = 4096;         // channels of a group: a row of them, with the partials, fits an SM
+
+inline dnb_status gn_shape_check(int64_t batch, int64_t spatial, int64_t filters, int64_t groups, const char *what) {
+    if (batch < 0 || spatial < 0 || filters <= 0 || groups <= 0)
+        return fail(DNB_ERR_INVALID, "%s: bad shape", what);
+    if (filters % groups) return fail(DNB_ERR_INVALID, "%s: groups must divide filters", what);
+    if (filters / groups > kGnMaxGroup)
+        return fail(DNB_ERR_UNSUPPORTED, "%s: more than %lld channels in a group", what, (long long)kGnMaxGroup);
+    const int64_t most = int64_t(1) << 44;  // elements: offsets stay far inside 63 bits
+    if (filters > most || (batch && spatial && (spatial > most / filters || batch > most / filters / spatial)))
+        return fail(DNB_ERR_INVALID, "%s: too large", what);
+    return DNB_OK;
+}
+
+inline int64_t gcd64(int64_t a, int64_t b) {
+    while (b) {
+        const int64_t t = a % b;
+        a = b;
+        b = t;
+    }
+    return a;
+}
+
+// tensors: inputs held in shared memory (1 forward, 2 or 3 backward); parts: per-thread partial arrays
+// (1 forward, 2 backward); align: the OR of the tensors' addresses.
+inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t groups, int64_t esize, uintptr_t align,
+                      int tensors, int parts) {
+    constexpr int sms = 148;  // a B200's; the plan must not depend on the current device, for the workspace's size
+    GnPlan p;
+    const int64_t cg = filters / groups;
+    const uintptr_t a = align | (uintptr_t)(filters * esize);
+    p.vb = a % 16 == 0 ? 16 : a % 4 == 0 ? 4 : (int)esize;
+    // groups that end on a vector's boundary; single elements where that makes units too wide to hold
+    if (p.vb / esize / gcd64(p.vb / esize, cg) * cg > kGnMaxGroup) p.vb = (int)esize;
+    const int64_t n = p.vb / esize;
+    const int64_t step = n / gcd64(n, cg);
+    auto cap = [&](int64_t g) { return g < groups ? g : groups; };
+    int64_t per = cap(step * ((64 + step * cg * esize - 1) / (step * cg * esize)));
+    auto slab_of = [&](int64_t g, int64_t rows) { return (size_t)((rows * g * cg * esize + 15) / 16 * 16); };
+    auto units_of = [&](int64_t g) { return batch * ((groups + g - 1) / g); };
+    // short planes: wider units, while they still fill the SMs twice
+    while (per < groups && cap(2 * per) * cg <= 2048 && slab_of(cap(2 * per), spatial) * tensors <= 16 * 1024 && units_of(cap(2 * per)) >= 2 * sms)
+        per = cap(2 * per);
+    // rows narrower than 64 bytes rather than a second read of the inputs
+    if (slab_of(per, (spatial + kGnMaxCluster - 1) / kGnMaxCluster) * tensors > kGnSmemMax && step < per) per = cap(step);
+    p.cb = per * cg;
+    p.nu = (groups + per - 1) / per;
+    auto shape = [&](int q) {
+        p.cluster = q;
+        p.rows = (spatial + q - 1) / q;
+        p.slab = slab_of(per, p.rows);
+        p.threads = p.slab * tensors > 64 * 1024 ? 512 : 256;
+        const int64_t v = p.cb / n;
+        p.part_floats = (size_t)(v >= p.threads ? p.cb : p.threads * n);  // of a narrower last unit too
+        // partial arrays; then per channel two floats, per group four doubles
+        p.smem = p.slab * tensors + p.part_floats * 4 * parts + (size_t)p.cb * 8 + (size_t)per * 32 + 64;
+    };
+    int q = 1;
+    shape(q);
+    while (q < kGnMaxCluster && p.smem > kGnSmemTarget) shape(q *= 2);
+    if (p.smem > kGnSmemMax) {
+        p.stream = true;
+        p.cluster = 1;
+        int64_t rows = (int64_t)(kGnStreamSlab / (size_t)(p.cb * esize * tensors));
+        if (rows < 1) rows = 1;
+        p.rows = rows;
+        p.chunks = (spatial + rows - 1) / rows;
+        const int64_t chunks = p.chunks;
+        // shared memory of a chunk: the partials alone where one row is all that fits
+        p.slab = slab_of(per, rows);
+        p.threads = 256;
+        const int64_t v = p.cb / n;
+        p.part_floats = (size_t)(v >= p.threads ? p.cb : p.threads * n);
+        p.smem = p.slab * tensors + p.part_floats * 4 * parts + (size_t)p.cb * 8 + (size_t)per * 32 + 64;
+        p.chunks = chunks;
+        return p;
+    }
+    // few units: more CTAs for each, while a CTA keeps 8 KB
+    while (q < kGnMaxCluster && units_of(per) * q < sms && p.slab * tensors > 16 * 1024) shape(q *= 2);
+    return p;
+}
+
+// ---- device helpers ----
+
+// Where a CTA works: unit, rows, columns.
+struct Place {
+    int64_t b, c0, r0;
+    int nr, cb, ng, g0;
+};
+template <class Args>
+__device__ __forceinline__ Place place_of(const Args &a, int64_t per_unit) {
+    Place p;
+    const int64_t unit = blockIdx.x / per_unit, q = blockIdx.x % per_unit;
+    p.b = unit / a.nu;
+    p.c0 = (unit % a.nu) * a.cb;
+    p.cb = (int)(a.cb < a.filters - p.c0 ? a.cb : a.filters - p.c0);
+    p.g0 = (int)(p.c0 / a.cg);
+    p.ng = (int)(p.cb / a.cg);
+    p.r0 = q * a.rows;
+    const int64_t left = a.spatial - p.r0;
+    p.nr = (int)(left < 0 ? 0 : left < a.rows ? left : a.rows);
+    return p;
+}
+
+__device__ __forceinline__ unsigned gn_cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void gn_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of `p` (shared memory) in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t gn_peer(const void *p, unsigned rank) {
+    uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ double gn_peer_f64(const void *p, unsigned rank) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(gn_peer(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float gn_peer_f32(const void *p, unsigned rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(gn_peer(p, rank)) : "memory");
+    return v;
+}
+
+// Launches a GN kernel with its shared memory and cluster size.
+template <class K, class Args>
+dnb_status gn_launch(K kernel, const Args &args, int64_t blocks, const GnPlan &p, const DeviceState *ds,
+                     cudaStream_t s, std::atomic<int> *opted, const char *what) {
+    if (!opted[ds->device].load(std::memory_order_acquire)) {
+        DNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ds->max_smem_optin));
+        opted[ds->device].store(1, std::memory_order_release);
+    }
+    if (blocks > 0x7fffffffll || p.smem > (size_t)ds->max_smem_optin)
+        return fail(DNB_ERR_UNSUPPORTED, "%s: too many units, or too many channels in a group", what);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)p.threads);
+    cfg.dynamicSmemBytes = p.smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+    DNB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
+    return after_launch(s, what);
+}
+
+}  // namespace dnb

@@ -1,0 +1,103 @@
+// Element types of the 16-bit entries: conversions, packed vectors of 16, 4 or one element's
+// bytes, and the host-side checks they share. Every 16-bit value is widened to fp32 exactly and
+// every result is rounded to nearest even once.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "dnb_common.cuh"
+
+namespace dnb {
+
+inline bool valid_dtype(int t) { return t == DNB_F32 || t == DNB_BF16 || t == DNB_F16; }
+inline bool valid_dtype16(int t) { return t == DNB_BF16 || t == DNB_F16; }
+inline int64_t dtype_size(int t) { return t == DNB_F32 ? 4 : 2; }
+
+// A matrix argument: `rows` rows of `cols` elements, `ld` elements apart. True if its size fits the
+// kernels' 63-bit byte arithmetic and its pointer is aligned to the element.
+inline bool matrix_ok(const void *p, int64_t rows, int64_t cols, int64_t ld, int dtype) {
+    const int64_t e = dtype_size(dtype);
+    if (reinterpret_cast<uintptr_t>(p) % (uintptr_t)e) return false;
+    if (rows <= 1) return rows <= 0 || (ld >= cols && cols <= (int64_t(1) << 60) / e);
+    return ld >= cols && ld <= (int64_t(1) << 60) / e / rows;
+}
+// Bytes from the matrix's first element to its last.
+inline int64_t matrix_span(int64_t rows, int64_t cols, int64_t ld, int64_t e) {
+    return rows <= 0 || cols <= 0 ? 0 : ((rows - 1) * ld + cols) * e;
+}
+inline bool overlaps(const void *a, int64_t an, const void *b, int64_t bn) {
+    if (!a || !b || an <= 0 || bn <= 0) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t)bn && y < x + (uintptr_t)an;
+}
+
+template <class T>
+struct Elem;
+template <>
+struct Elem<float> {
+    static __device__ __forceinline__ float to(float v) { return v; }
+    static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+    static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Elem<__half> {
+    static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+};
+
+// VB bytes of elements moved by one access.
+template <int VB>
+struct RawVec;
+template <>
+struct RawVec<16> { using type = uint4; };
+template <>
+struct RawVec<8> { using type = uint2; };
+template <>
+struct RawVec<4> { using type = uint32_t; };
+template <>
+struct RawVec<2> { using type = uint16_t; };
+
+template <class T, int VB>
+struct Vec {
+    static constexpr int N = VB / (int)sizeof(T);
+    using Raw = typename RawVec<VB>::type;
+    union U {
+        Raw raw;
+        T e[N];
+        __device__ U() {}
+    };
+    static __device__ __forceinline__ void unpack(const Raw &r, float (&f)[N]) {
+        U u;
+        u.raw = r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = Elem<T>::to(u.e[i]);
+    }
+    static __device__ __forceinline__ Raw pack(const float (&f)[N]) {
+        U u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) u.e[i] = Elem<T>::from(f[i]);
+        return u.raw;
+    }
+};
+
+// Calls f.template operator()<T>() with the element type.
+template <class F>
+auto dispatch_dtype(int dtype, F &&f) {
+    switch (dtype) {
+    case DNB_BF16: return f.template operator()<__nv_bfloat16>();
+    case DNB_F16: return f.template operator()<__half>();
+    default: return f.template operator()<float>();
+    }
+}
+template <class F>
+auto dispatch_dtype16(int dtype, F &&f) {
+    if (dtype == DNB_BF16) return f.template operator()<__nv_bfloat16>();
+    return f.template operator()<__half>();
+}
+
+}  // namespace dnb

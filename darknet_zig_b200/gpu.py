@@ -8,6 +8,9 @@ no gpu.zig counterpart follow after the mirrored ones.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+
 import torch
 
 from ._lib import DnbError, call, lib  # noqa: F401  (DnbError re-exported)
@@ -248,6 +251,124 @@ def sgdMomentum(n, weights, weight_updates, learning_rate, momentum, decay, batc
 def softmaxXent(input, truth, n, batch, temp, output, delta, err, cost=None):  # noqa: N802,A002
     call("softmax_xent", _p(input), _p(truth), int(n), int(batch), float(temp), _p(output), _p(delta), _p(err),
          _p(cost), _s())
+
+
+# ---- 16-bit training and serving path (no reference counterparts; see include/dnb200.h) ----
+#
+# These take tensors instead of pointers and sizes alone: each argument is checked for its type, device
+# and shape, and a matrix may have rows that are further apart than they are long (a view of a wider
+# tensor). `workspace` (a uint8 CUDA tensor of at least the entry's *_workspace bytes) keeps the call
+# free of allocations; None takes one from torch's allocator, which is safe under graph capture too.
+
+F32, BF16, F16 = range(3)
+DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+ACC_UPDATES, ACC_DELTA = 1, 2
+
+
+def _on_device(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name}: expected a CUDA tensor")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _dtype(t, name, allowed=(torch.bfloat16, torch.float16)):
+    if not isinstance(t, torch.Tensor) or t.dtype not in allowed:
+        raise TypeError(f"{name}: expected one of {allowed}, got {getattr(t, 'dtype', type(t))}")
+    return DTYPES[t.dtype]
+
+
+def _vec(t, name, n, dtype=torch.float32, optional=False):
+    """Pointer of a contiguous vector of n elements."""
+    if t is None and optional:
+        return None
+    _on_device(t, name)
+    if t.dtype != dtype or not t.is_contiguous() or t.numel() != n:
+        raise ValueError(f"{name}: expected {n} contiguous {dtype} elements, got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def _mat(t, name, rows, cols, dtype, optional=False):
+    """(pointer, row stride) of a matrix: a [rows, cols] view with unit column stride, or any contiguous
+    tensor of rows * cols elements."""
+    if t is None and optional:
+        return None, cols
+    _on_device(t, name)
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols and (t.stride(1) == 1 or cols <= 1) and (
+            rows <= 1 or t.stride(0) >= cols):
+        return t.data_ptr(), max(t.stride(0), cols) if rows > 1 else cols
+    if t.is_contiguous() and t.numel() == rows * cols:
+        return t.data_ptr(), cols
+    raise ValueError(f"{name}: expected a [{rows}, {cols}] matrix with contiguous rows, got {tuple(t.shape)} with "
+                     f"strides {t.stride()}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, args):
+    n = ctypes.c_size_t(0)
+    call(name, *args, ctypes.byref(n))
+    return int(n.value)
+
+
+def _align(p):
+    """A stand-in for a pointer in a workspace query, which looks at alignment (and NULL) only."""
+    return None if p is None else 16 + (p & 15)
+
+
+def _workspace(workspace, name, *args):
+    """(pointer, bytes) of the given workspace or of one that torch allocates, with the tensor that holds it.
+    The caller keeps the tensor until the launch; torch orders its reuse on the current stream."""
+    if workspace is not None:
+        _on_device(workspace, "workspace")
+        if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise TypeError("workspace: expected a contiguous uint8 tensor")
+        return workspace.data_ptr(), workspace.numel(), workspace
+    n = _workspace_bytes(name, args)
+    if n == 0:
+        return None, 0, None
+    t = torch.empty(n, dtype=torch.uint8, device="cuda")
+    return t.data_ptr(), n, t
+
+
+def gnActForward(x, y, batch, spatial, filters, groups, scales, biases, eps, mean, rstd, act,  # noqa: N802
+                 workspace=None):
+    """Group norm + activation on a channels-last tensor [batch, spatial, filters] (f32, bf16 or f16)."""
+    dt = _dtype(x, "x", tuple(DTYPES))
+    n = batch * spatial * filters
+    px, py = _vec(x, "x", n, x.dtype), _vec(y, "y", n, x.dtype)
+    ws, wn, _keep = _workspace(workspace, "gn_act_forward_workspace", _align(px), _align(py), dt, batch, spatial,
+                               filters, groups)
+    call("gn_act_forward", px, py, dt, batch, spatial, filters, groups, _vec(scales, "scales", filters),
+         _vec(biases, "biases", filters), eps, _vec(mean, "mean", batch * groups),
+         _vec(rstd, "rstd", batch * groups), act, ws, wn, _s())
+
+
+def gnActBackward(x, y, delta, dx, batch, spatial, filters, groups, scales, biases, mean, rstd,  # noqa: N802
+                  bias_updates, scale_updates, act, accumulate=ACC_UPDATES, workspace=None):
+    """Backward of gnActForward; y may be None (recomputed). The updates are added to unless accumulate=0."""
+    dt = _dtype(x, "x", tuple(DTYPES))
+    n = batch * spatial * filters
+    px, py = _vec(x, "x", n, x.dtype), _vec(y, "y", n, x.dtype, optional=True)
+    pd, pdx = _vec(delta, "delta", n, x.dtype), _vec(dx, "dx", n, x.dtype)
+    ws, wn, _keep = _workspace(workspace, "gn_act_backward_workspace", _align(px), _align(py), _align(pd),
+                               _align(pdx), dt, batch, spatial, filters, groups)
+    call("gn_act_backward", px, py, pd, pdx, dt, batch, spatial, filters, groups, _vec(scales, "scales", filters),
+         _vec(biases, "biases", filters), _vec(mean, "mean", batch * groups), _vec(rstd, "rstd", batch * groups),
+         _vec(bias_updates, "bias_updates", filters), _vec(scale_updates, "scale_updates", filters), act, accumulate,
+         ws, wn, _s())
+
+
+def sgdMomentumMixed(weights, weight_updates, gradients, weights16, rows, cols, learning_rate, momentum,  # noqa: N802
+                     decay, batch):
+    """sgdMomentum with 16-bit gradients in (None: already in weight_updates) and 16-bit weights out."""
+    dt = _dtype(weights16, "weights16")
+    g, ldg = _mat(gradients, "gradients", rows, cols, weights16.dtype, optional=True)
+    w16, ld16 = _mat(weights16, "weights16", rows, cols, weights16.dtype)
+    call("sgd_momentum_mixed", rows, cols, _vec(weights, "weights", rows * cols),
+         _vec(weight_updates, "weight_updates", rows * cols), g, ldg, w16, ld16, dt, learning_rate, momentum, decay,
+         batch, _s())
 
 
 # ---- fused sync-BN across GPUs (no reference counterpart) --------------------------------

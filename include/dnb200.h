@@ -372,6 +372,82 @@ dnb_status dnb_syncbn_backward_apply(const float *x, const float *y, const float
                                      const float *variance, float *bias_updates, float *scale_updates,
                                      float *mean_delta, float *variance_delta, int act, dnb_stream stream);
 
+/* ------------------------------------------------------------------------------------ */
+/* 16-bit training and serving path: group norm + activation on channels-last tensors,    */
+/* the connected layer (product, bias, residual, activation) with its backward, softmax   */
+/* cross entropy from the connected layer's inputs, and the SGD update that keeps a 16-bit */
+/* copy of fp32 weights. No counterparts in the reference, whose tensors are all fp32; the */
+/* layer each stands beside is named at its entry.                                        */
+/*                                                                                        */
+/* Conventions of this section:                                                           */
+/*   - tensors are row-major matrices of `dtype` elements; a channels-last tensor           */
+/*     [batch][spatial][filters] is a matrix of batch*spatial rows, so the rows of a group  */
+/*     norm are the rows of a connected layer (a 1x1 convolution). ld* is the distance      */
+/*     between row starts in elements (>= the row's length); elements between a row's end   */
+/*     and the next row's start are neither read nor written;                               */
+/*   - biases, scales, statistics, losses and bias / scale updates are fp32;                */
+/*   - sums, statistics and products are accumulated in fp32 or fp64, and each output is    */
+/*     rounded once unless its entry says otherwise;                                       */
+/*   - pointers must be aligned to their element. Rows that start on 16-byte boundaries     */
+/*     (pointer and ld) take the fast paths: the others work, through narrower accesses or  */
+/*     an aligned copy in the workspace;                                                   */
+/*   - scratch memory is the caller's: dnb_*_workspace says how many bytes the call with    */
+/*     the same arguments needs (0 = workspace may be NULL). The workspace must be 16-byte  */
+/*     aligned, needs no initialisation, and belongs to the call until its work on the      */
+/*     stream is done: concurrent calls, and graphs that may replay concurrently, need one  */
+/*     each. No call allocates, synchronises or touches the library's own workspaces, so    */
+/*     every one may be captured into a graph;                                             */
+/*   - an output may not overlap an input or another output, except where its entry says    */
+/*     that it may be the same tensor (same pointer and ld);                               */
+/*   - results do not depend on timing: the same call gives the same bits on the same GPU   */
+/*     model.                                                                              */
+/* ------------------------------------------------------------------------------------ */
+
+/* element types */
+enum { DNB_F32 = 0, DNB_BF16 = 1, DNB_F16 = 2 };
+/* bits of `accumulate`: add to what the updates / the input delta hold (as the reference's
+ * layers do) instead of overwriting it */
+enum { DNB_ACC_UPDATES = 1, DNB_ACC_DELTA = 2 };
+
+/* Group norm + activation, training or inference (beside batchnorm.forward, batchnorm.zig:129-153,
+ * whose statistics depend on the batch; these do not). x, y: [batch][spatial][filters] of dtype
+ * (f32, bf16, f16); the `groups` groups are runs of filters/groups channels (filters % groups == 0).
+ * Per (image, group), over its n = spatial * filters/groups elements:
+ *   mean = sum(x)/n;  rstd = 1/sqrt(sum((x - mean)^2)/n + eps)  (biased variance);
+ *   y = act(((x - mean) * rstd) * scales[c] + biases[c]).
+ * mean, rstd: out, [batch][groups], kept for the backward. eps >= 0. y may be x. batch or spatial 0:
+ * nothing is written. A group of more than 4096 channels: DNB_ERR_UNSUPPORTED. */
+dnb_status dnb_gn_act_forward(const void *x, void *y, int dtype, int64_t batch, int64_t spatial, int64_t filters,
+                              int64_t groups, const float *scales, const float *biases, float eps, float *mean,
+                              float *rstd, int act, void *workspace, size_t workspace_bytes, dnb_stream stream);
+dnb_status dnb_gn_act_forward_workspace(const void *x, const void *y, int dtype, int64_t batch, int64_t spatial,
+                                        int64_t filters, int64_t groups, size_t *bytes);
+/* Backward of dnb_gn_act_forward (beside batchnorm.backward, batchnorm.zig:155-169). x: the forward's
+ * input; mean, rstd: its statistics; delta = dL/dy; y: the forward's output, from which the activation's
+ * gradient is taken; NULL = the output is recomputed from x in fp32.
+ *   d = delta * act'(y);  t = d * scales[c];  xh = (x - mean) * rstd;
+ *   dx = rstd * (t - sum(t)/n - xh * sum(t*xh)/n)   (dx may be delta);
+ *   bias_updates[c] (+)= sum(d);  scale_updates[c] (+)= sum(d * xh)   (added with DNB_ACC_UPDATES). */
+dnb_status dnb_gn_act_backward(const void *x, const void *y, const void *delta, void *dx, int dtype, int64_t batch,
+                               int64_t spatial, int64_t filters, int64_t groups, const float *scales,
+                               const float *biases, const float *mean, const float *rstd, float *bias_updates,
+                               float *scale_updates, int act, int accumulate, void *workspace,
+                               size_t workspace_bytes, dnb_stream stream);
+dnb_status dnb_gn_act_backward_workspace(const void *x, const void *y, const void *delta, const void *dx, int dtype,
+                                         int64_t batch, int64_t spatial, int64_t filters, int64_t groups,
+                                         size_t *bytes);
+
+/* SGD with momentum and decay on fp32 weights (dnb_sgd_momentum) with 16-bit gradients in and a 16-bit
+ * copy of the weights out, in one pass over [rows][cols]:
+ *   wu += gradients;  wu += (-decay*batch) * w;  w += (learning_rate/batch) * wu;  wu *= momentum;
+ *   weights16 = w rounded to dtype (bf16 or f16).
+ * weights, weight_updates: contiguous fp32. gradients (row stride ldg) may be NULL: the gradients have
+ * been added to weight_updates already. weights16 has row stride ld16. gradients may be weights16. */
+dnb_status dnb_sgd_momentum_mixed(int64_t rows, int64_t cols, float *weights, float *weight_updates,
+                                  const void *gradients, int64_t ldg, void *weights16, int64_t ld16, int dtype,
+                                  float learning_rate, float momentum, float decay, int64_t batch,
+                                  dnb_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,80 @@
+"""Arguments that the 16-bit entries refuse, on the CPU: the status comes back before a device is touched."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+
+from darknet_zig_b200 import _lib
+
+F32, BF16, F16 = 0, 1, 2
+P = 1 << 20  # a stand-in for a device pointer; never dereferenced
+INVALID, UNSUPPORTED = 1, 5
+
+
+def status(name, *args):
+    L = _lib.lib()
+    fn = getattr(L, "dnb_" + name)
+    assert len(fn.argtypes) == len(args), (name, len(fn.argtypes), len(args))
+    st = fn(*args)
+    if st:
+        assert L.dnb_last_error_detail()
+    return st
+
+
+def gn_fwd(x=P, y=2 * P, dtype=BF16, B=2, S=4, Cn=8, G=2, sc=3 * P, bi=4 * P, eps=1e-5, mean=5 * P, rstd=6 * P, act=7,
+           ws=None, wn=0):
+    return status("gn_act_forward", x, y, dtype, B, S, Cn, G, sc, bi, eps, mean, rstd, act, ws, wn, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=3), dict(dtype=-1), dict(B=-1), dict(S=-1), dict(Cn=0), dict(G=0), dict(G=3), dict(act=14),
+    dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(y=None), dict(sc=None), dict(bi=None), dict(mean=None),
+    dict(rstd=None), dict(x=P + 1), dict(y=P + 16), dict(rstd=5 * P + 4), dict(mean=P), dict(B=1 << 40, S=1 << 40),
+])
+def test_gn_forward_refuses(built_lib, kw):
+    assert gn_fwd(**kw) == INVALID
+
+
+def test_gn_refuses_wide_groups_and_short_workspaces(built_lib):
+    assert gn_fwd(Cn=8192, G=1) == UNSUPPORTED
+    n = C.c_size_t(0)
+    args = (BF16, 1, 1 << 20, 64, 1)
+    assert status("gn_act_forward_workspace", P, 2 * P, *args, C.byref(n)) == 0 and n.value > 0
+    big = dict(B=1, S=1 << 20, Cn=64, G=1, y=1 << 40, mean=1 << 41, rstd=1 << 42)
+    assert gn_fwd(**big) == INVALID
+    assert gn_fwd(**big, ws=1 << 43, wn=n.value - 1) == INVALID
+    assert gn_fwd(**big, ws=(1 << 43) + 8, wn=n.value) == INVALID
+    assert status("gn_act_forward_workspace", P, 2 * P, *args, None) == INVALID
+
+
+def gn_bwd(x=P, y=None, d=2 * P, dx=3 * P, dtype=BF16, B=2, S=4, Cn=8, G=2, sc=4 * P, bi=5 * P, mean=6 * P, rstd=7 * P,
+           bu=8 * P, su=9 * P, act=7, acc=0, ws=10 * P, wn=1 << 19):
+    return status("gn_act_backward", x, y, d, dx, dtype, B, S, Cn, G, sc, bi, mean, rstd, bu, su, act, acc, ws, wn, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=9), dict(B=-1), dict(G=3), dict(act=-1), dict(acc=2), dict(acc=5), dict(x=None), dict(d=None),
+    dict(dx=None), dict(sc=None), dict(bi=None), dict(mean=None), dict(rstd=None), dict(bu=None), dict(su=None),
+    dict(dx=P), dict(y=3 * P), dict(dx=2 * P + 32), dict(su=8 * P + 4), dict(x=P + 1), dict(ws=None), dict(wn=1),
+    dict(ws=10 * P + 4), dict(bu=3 * P),
+])
+def test_gn_backward_refuses(built_lib, kw):
+    assert gn_bwd(**kw) == INVALID
+
+
+def sgd(rows=4, cols=8, w=P, wu=2 * P, g=3 * P, ldg=8, w16=4 * P, ld16=8, dtype=BF16, batch=4):
+    return status("sgd_momentum_mixed", rows, cols, w, wu, g, ldg, w16, ld16, dtype, 0.1, 0.9, 0.0, batch, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(rows=-1), dict(cols=-1), dict(dtype=F32), dict(batch=0), dict(w=None), dict(wu=None), dict(w16=None),
+    dict(ldg=7), dict(ld16=7), dict(w=P + 2), dict(w16=4 * P + 1), dict(wu=P + 64), dict(w16=P), dict(g=2 * P),
+    dict(g=4 * P, ldg=9), dict(rows=1 << 40, cols=1 << 40, ldg=1 << 40, ld16=1 << 40),
+])
+def test_sgd_refuses(built_lib, kw):
+    assert sgd(**kw) == INVALID
+
+
+def test_sgd_of_nothing(built_lib):
+    assert sgd(rows=0) == 0 and sgd(cols=0, w=None) == 0
