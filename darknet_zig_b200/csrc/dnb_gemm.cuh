@@ -1,0 +1,424 @@
+// The matrix product behind the connected layer and the cross entropy: C[m][n] = sum_k A(m,k) B(n,k) with
+// 16-bit operands and fp32 accumulators on the 5th-generation tensor cores, persistent, with the epilogue
+// as a template argument.
+//
+// An operand is K-major (its rows run along k: x and w of a forward product) or MN-major (its rows run
+// along m or n: the transposed operands of a backward product); both are brought in by TMA with the
+// 128-byte swizzle and described to the tensor core where they lie, so no product needs a transposed copy.
+//
+// A CTA (CTAS = 1) or a pair on neighbouring SMs (CTAS = 2, cta_group::2) owns one output tile of
+// 128*CTAS x BN at a time. Warp 0 issues the loads into a ring of stages (64 k each), warp 1 of the pair's
+// first CTA issues the products into one of two accumulators in tensor memory, warps 4-7 take the other
+// accumulator through the epilogue meanwhile. A pair halves the operand traffic per SM: each CTA holds its
+// own 128 rows of A and half of B's rows, and the products read both CTAs' shared memory.
+//
+// Every wait is bounded (dnb_set_wait_limit_ms): a role whose wait gives up sets the error word and
+// leaves its loop; the others' waits then end the same way, the CTA (pair) meets at its last barrier and
+// frees its tensor memory.
+#pragma once
+
+#include <cuda.h>
+
+#include <atomic>
+
+#include "dnb_types.cuh"
+
+namespace dnb {
+
+// ---- host side: tensor maps ----
+
+// A 2-D tensor map of 16-bit elements: `inner` contiguous elements, `outer` rows `stride` elements apart,
+// boxes of 64 x box_outer elements with the 128-byte swizzle, zeros outside. dnb_gemm.cu.
+dnb_status make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t outer, int64_t stride, int box_outer,
+                    int dtype, const char *what);
+
+// An operand as the tensor core wants it: 16-byte aligned rows. `mn` rows of length k (K-major), or k rows
+// of length mn (MN-major).
+struct Operand {
+    const void *p = nullptr;
+    int64_t ld = 0;
+};
+inline bool tma_ready(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
+// ---- the product's description ----
+
+struct GemmArgs {
+    int64_t m, n, k;
+    int m_tiles, n_tiles, k_blocks;
+    int band;       // output tiles are taken in bands of this many row tiles, down the rows first
+    unsigned idesc; // the tensor core's instruction descriptor
+    unsigned long long wait_ns;
+    unsigned *error_word;
+};
+
+constexpr int kGemmThreads = 256;
+constexpr int kBlockK = 64;
+constexpr unsigned DEVERR_WAIT_GEMM = 8u;  // a role of a product gave up waiting
+
+template <int CTAS_, int BN_, bool A_MN_, bool B_MN_>
+struct GemmCfg {
+    static constexpr int CTAS = CTAS_, BN = BN_;
+    static constexpr bool A_MN = A_MN_, B_MN = B_MN_;
+    static constexpr int BM = 128;             // rows of one CTA
+    static constexpr int TM = BM * CTAS;       // rows of a tile
+    static constexpr int BROWS = BN / CTAS;    // B rows one CTA holds
+    static constexpr int A_BYTES = BM * kBlockK * 2, B_BYTES = BROWS * kBlockK * 2;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = STAGE >= 32768 ? 6 : STAGE >= 24576 ? 8 : 9;
+    static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 256;
+    static_assert(BN % 32 == 0 && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
+    static_assert(!B_MN || BROWS % 64 == 0, "an MN-major box is 64 wide");
+};
+
+// ---- device side ----
+
+namespace gemm {
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {  // bar: a shared::cluster address
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 0x989680;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Waits for the phase of `parity` to end. False: the limit passed or another role gave up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const GemmArgs &g, volatile unsigned *gave_up) {
+    if (mbar_try(bar, parity)) return true;
+    const unsigned long long start = global_ns();
+    while (!mbar_try(bar, parity)) {
+        if (*gave_up) return false;
+        if (global_ns() - start > g.wait_ns) {
+            *gave_up = 1u;
+            atomicOr(g.error_word, DEVERR_WAIT_GEMM);
+            return false;
+        }
+    }
+    return true;
+}
+
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One box of a tensor map into this CTA's shared memory; `bar` (a shared::cluster address) counts its bytes.
+template <int CTAS>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+            "[%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+            "[%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle. K-major: rows of 128 bytes, 8-row groups 1024 bytes
+// apart (stride offset); the leading offset is unused. MN-major: 64-element runs along mn, 8-k groups 1024
+// bytes apart (stride offset), 64-wide column blocks `leading` bytes apart.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <int CTAS>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add)
+            : "memory");
+}
+// Arrives on `bar` (in both CTAs of a pair) when the products issued so far are done.
+template <int CTAS>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+                     : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
+    if constexpr (CTAS == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
+    if constexpr (CTAS == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes: v[j] is (lane, column j).
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+}
+
+// The row tile and column tile of the t-th tile.
+__device__ __forceinline__ void tile_at(const GemmArgs &g, int t, int &mt, int &nt) {
+    const int per = g.band * g.n_tiles, b = t / per, in = t - b * per;
+    const int rows = min(g.band, g.m_tiles - b * g.band);
+    nt = in / rows;
+    mt = b * g.band + (in - nt * rows);
+}
+
+}  // namespace gemm
+
+// Epi: a struct passed by value to the kernel, with
+//   struct State;                                          a thread's row, kept over a tile's columns
+//   void begin(State &, int64_t row, int64_t col0) const;
+//   void columns(State &, float (&v)[32], int64_t row, int64_t col) const;   32 columns from `col`
+//   void end(State &, int64_t row, int64_t col0) const;
+// All 32 lanes call each of them (rows beyond m included: the functions check).
+template <class C, class Epi>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+           const __grid_constant__ GemmArgs g, const __grid_constant__ Epi epi) {
+    using namespace gemm;
+    constexpr int CTAS = C::CTAS, S = C::STAGES;
+    extern __shared__ unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char *tail = raw + (base - smem_u32(raw)) + S * C::STAGE;
+    // barriers after the stages: full[S], empty[S], accumulator full[2], accumulator empty[2]; then the
+    // tensor memory's address and the give-up flag
+    const uint32_t bars = base + S * C::STAGE;
+    const uint32_t full = bars, empty = bars + 8 * S, acc_full = bars + 16 * S, acc_empty = acc_full + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 16 * S + 32);
+    volatile unsigned *gave_up = reinterpret_cast<volatile unsigned *>(tail + 16 * S + 36);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CTAS == 2 ? cluster_rank() : 0u;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full + 8 * b, 1);
+            mbar_init(acc_empty + 8 * b, 4 * CTAS);
+        }
+        *gave_up = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    if (warp == 2) tmem_alloc<CTAS>(smem_u32(tmem_slot), C::TMEM_COLS);
+    fence_before();
+    __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int tiles = g.m_tiles * g.n_tiles, step = (int)gridDim.x / CTAS, first = (int)blockIdx.x / CTAS;
+
+    if (warp == 0 && lane == 0) {
+        // loads
+        int it = 0;
+        bool ok = true;
+        for (int t = first; ok && t < tiles; t += step) {
+            int mt, nt;
+            tile_at(g, t, mt, nt);
+            const int am = mt * C::TM + (int)rank * C::BM, bn = nt * C::BN + (int)rank * C::BROWS;
+            for (int kb = 0; kb < g.k_blocks; ++kb, ++it) {
+                const int s = it % S;
+                if (!mbar_wait(empty + 8 * s, ((it / S) & 1) ^ 1, g, gave_up)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t a_at = base + s * C::STAGE, b_at = a_at + C::A_BYTES;
+                const uint32_t bar = CTAS == 2 ? map_rank(full + 8 * s, 0) : full + 8 * s;
+                if (rank == 0) mbar_expect(full + 8 * s, C::STAGE * CTAS);
+                const int k0 = kb * kBlockK;
+                if constexpr (C::A_MN) {
+#pragma unroll
+                    for (int c = 0; c < C::BM / 64; ++c) tma_load<CTAS>(a_at + c * 8192, &map_a, am + c * 64, k0, bar);
+                } else {
+                    tma_load<CTAS>(a_at, &map_a, k0, am, bar);
+                }
+                if constexpr (C::B_MN) {
+#pragma unroll
+                    for (int c = 0; c < C::BROWS / 64; ++c)
+                        tma_load<CTAS>(b_at + c * 8192, &map_b, bn + c * 64, k0, bar);
+                } else {
+                    tma_load<CTAS>(b_at, &map_b, k0, bn, bar);
+                }
+            }
+        }
+        // the last products still read (and their commits still arrive at) these stages
+        for (int j = it > S ? it - S : 0; ok && j < it; ++j)
+            if (!mbar_wait(empty + 8 * (j % S), (j / S) & 1, g, gave_up)) ok = false;
+        // giving up: the copies in flight still land in this pair's shared memory (each try sleeps up to 10 ms)
+        if (!ok && rank == 0)
+            for (int j = it > S ? it - S : 0; j < it; ++j)
+                for (int tries = 0; tries < 20 && !mbar_try(full + 8 * (j % S), (j / S) & 1); ++tries) {}
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // products
+        int it = 0, n = 0;
+        bool ok = true;
+        for (int t = first; ok && t < tiles; t += step, ++n) {
+            const int b = n & 1;
+            if (!mbar_wait(acc_empty + 8 * b, ((n >> 1) & 1) ^ 1, g, gave_up)) break;
+            fence_after();
+            const uint32_t d = tmem + b * C::BN;
+            for (int kb = 0; kb < g.k_blocks; ++kb, ++it) {
+                const int s = it % S;
+                if (!mbar_wait(full + 8 * s, (it / S) & 1, g, gave_up)) {
+                    ok = false;
+                    break;
+                }
+                fence_after();
+                const uint32_t a_at = base + s * C::STAGE, b_at = a_at + C::A_BYTES;
+                const uint64_t da = smem_desc(a_at, C::A_MN ? 8192u : 16u), db = smem_desc(b_at, C::B_MN ? 8192u : 16u);
+#pragma unroll
+                for (int k = 0; k < kBlockK / 16; ++k)  // 16 k: 32 bytes of a K-major row, 16 rows MN-major
+                    mma<CTAS>(d, da + (uint64_t)(k * (C::A_MN ? 2048 : 32) >> 4),
+                              db + (uint64_t)(k * (C::B_MN ? 2048 : 32) >> 4), g.idesc, (kb | k) != 0);
+                commit<CTAS>(empty + 8 * s);
+            }
+            if (ok) commit<CTAS>(acc_full + 8 * b);
+        }
+    } else if (warp >= 4) {
+        // epilogue: warp w reads tensor-memory lanes 32w..32w+31, a lane per row
+        const int w = warp - 4;
+        int n = 0;
+        for (int t = first; t < tiles; t += step, ++n) {
+            const int b = n & 1;
+            int mt, nt;
+            tile_at(g, t, mt, nt);
+            const bool ok = mbar_wait(acc_full + 8 * b, (n >> 1) & 1, g, gave_up);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            fence_after();
+            const int64_t row = (int64_t)mt * C::TM + (int64_t)rank * C::BM + w * 32 + lane, col0 = (int64_t)nt * C::BN;
+            const uint32_t at = tmem + ((uint32_t)(w * 32) << 16) + b * C::BN;
+            typename Epi::State st;
+            epi.begin(st, row, col0);
+#pragma unroll 1
+            for (int c = 0; c < C::BN; c += 32) {
+                if (col0 + c >= g.n) break;
+                float v[32];
+                tmem_load32(at + c, v);
+                epi.columns(st, v, row, col0 + c);
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(CTAS == 2 ? map_rank(acc_empty + 8 * b, 0) : acc_empty + 8 * b);
+            epi.end(st, row, col0);
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();
+    fence_after();
+    if (warp == 2) tmem_free<CTAS>(tmem, C::TMEM_COLS);
+}
+
+// Launches the product of a and b (already TMA-ready).
+template <class C, class Epi>
+dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k, const Epi &epi,
+                       const DeviceState *ds, cudaStream_t s, const char *what) {
+    static std::atomic<int> opted[kMaxDevices];
+    auto kernel = k_gemm<C, Epi>;
+    if (!opted[ds->device].load(std::memory_order_acquire)) {
+        DNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+        opted[ds->device].store(1, std::memory_order_release);
+    }
+    CUtensorMap ma, mb;
+    if (C::A_MN) DNB_TRY(make_map(&ma, a.p, m, k, a.ld, 64, dtype, what));
+    else DNB_TRY(make_map(&ma, a.p, k, m, a.ld, C::BM, dtype, what));
+    if (C::B_MN) DNB_TRY(make_map(&mb, b.p, n, k, b.ld, 64, dtype, what));
+    else DNB_TRY(make_map(&mb, b.p, k, n, b.ld, C::BROWS, dtype, what));
+    GemmArgs g;
+    g.m = m;
+    g.n = n;
+    g.k = k;
+    const int64_t mt = (m + C::TM - 1) / C::TM, nt = (n + C::BN - 1) / C::BN;
+    if (mt * nt > 0x3fffffffll) return fail(DNB_ERR_UNSUPPORTED, "%s: too many output tiles", what);
+    g.m_tiles = (int)mt;
+    g.n_tiles = (int)nt;
+    g.k_blocks = (int)((k + kBlockK - 1) / kBlockK);
+    g.band = 8;
+    // fp32 accumulators; operand type; majors; n / 8; m / 16
+    const unsigned t = dtype == DNB_BF16 ? 1u : 0u;
+    g.idesc = (1u << 4) | (t << 7) | (t << 10) | ((C::A_MN ? 1u : 0u) << 15) | ((C::B_MN ? 1u : 0u) << 16) |
+              ((unsigned)(C::BN / 8) << 17) | ((unsigned)(C::TM / 16) << 24);
+    g.wait_ns = wait_limit_ns();
+    g.error_word = ds->error_word;
+    const int64_t slots = ds->sm_count / C::CTAS, tiles = mt * nt;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((tiles < slots ? tiles : slots) * C::CTAS));
+    cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = C::CTAS;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = C::CTAS > 1 ? 1 : 0;
+    DNB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, g, epi));
+    return after_launch(s, what);
+}
+
+}  // namespace dnb

@@ -371,6 +371,49 @@ def sgdMomentumMixed(weights, weight_updates, gradients, weights16, rows, cols, 
          batch, _s())
 
 
+def connectedActForward(x, w, biases, residual, y, batch, inputs, outputs, act, workspace=None):  # noqa: N802
+    """y = act(x w^T + biases + residual); x [batch, inputs], w [outputs, inputs], residual (None, or y itself)
+    and y [batch, outputs] of bf16 or f16, biases fp32 or None."""
+    dt = _dtype(x, "x")
+    px, ldx = _mat(x, "x", batch, inputs, x.dtype)
+    pw, ldw = _mat(w, "w", outputs, inputs, x.dtype)
+    pr, ldr = _mat(residual, "residual", batch, outputs, x.dtype, optional=True)
+    py, ldy = _mat(y, "y", batch, outputs, x.dtype)
+    ws, wn, _keep = _workspace(workspace, "connected_act_forward_workspace", _align(px), ldx, _align(pw), ldw, dt,
+                               batch, inputs, outputs)
+    call("connected_act_forward", px, ldx, pw, ldw, _vec(biases, "biases", outputs, optional=True), pr, ldr, py, ldy,
+         dt, batch, inputs, outputs, act, ws, wn, _s())
+
+
+def connectedActBackward(x, w, y, delta, dz, dx, bias_updates, weight_updates, batch, inputs, outputs,  # noqa: N802
+                         act, accumulate=ACC_UPDATES, workspace=None):
+    """Backward of connectedActForward: dz = delta * act'(y) (None for linear, where it is delta; may be delta),
+    dx, weight_updates (x's type or fp32) and bias_updates (fp32), each of the three None if not wanted. The
+    updates are added to unless accumulate lacks ACC_UPDATES; dx is overwritten unless it has ACC_DELTA."""
+    dt = _dtype(x, "x")
+    px, ldx = _mat(x, "x", batch, inputs, x.dtype)
+    pw, ldw = _mat(w, "w", outputs, inputs, x.dtype)
+    py, ldy = _mat(y, "y", batch, outputs, x.dtype, optional=True)
+    pd, ldd = _mat(delta, "delta", batch, outputs, x.dtype)
+    pz, ldz = _mat(dz, "dz", batch, outputs, x.dtype, optional=True)
+    pdx, lddx = _mat(dx, "dx", batch, inputs, x.dtype, optional=True)
+    pu, ldu, ut = _updates(weight_updates, outputs, inputs, x.dtype)
+    ws, wn, _keep = _workspace(workspace, "connected_act_backward_workspace", _align(px), ldx, _align(pw), ldw,
+                               _align(pd), ldd, _align(pz), ldz, dt, batch, inputs, outputs, act)
+    call("connected_act_backward", px, ldx, pw, ldw, py, ldy, pd, ldd, pz, ldz, pdx, lddx,
+         _vec(bias_updates, "bias_updates", outputs, optional=True), pu, ldu, ut, dt, batch, inputs, outputs, act,
+         accumulate, ws, wn, _s())
+
+
+def _updates(t, rows, cols, dtype):
+    """(pointer, row stride, type) of weight updates: the operands' type or fp32."""
+    if t is None:
+        return None, cols, F32
+    ut = _dtype(t, "weight_updates", (dtype, torch.float32))
+    p, ld = _mat(t, "weight_updates", rows, cols, t.dtype)
+    return p, ld, ut
+
+
 # ---- fused sync-BN across GPUs (no reference counterpart) --------------------------------
 
 def commInit(rank: int, world: int, max_channels: int):  # noqa: N802

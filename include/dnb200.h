@@ -448,6 +448,37 @@ dnb_status dnb_sgd_momentum_mixed(int64_t rows, int64_t cols, float *weights, fl
                                   float learning_rate, float momentum, float decay, int64_t batch,
                                   dnb_stream stream);
 
+/* The connected layer (connected.zig:92-119 and, for channels-last tensors, the 1x1 convolution) with the
+ * shortcut layer's addition (misc.zig:244-270) and the activation in the product's epilogue:
+ *   y[m][n] = act(sum_k x[m][k] * w[n][k] + biases[n] + residual[m][n]).
+ * x [batch][inputs], w [outputs][inputs], residual and y [batch][outputs] of dtype (bf16 or f16).
+ * biases and residual may be NULL. y may be the residual. inputs == 0: the sum is 0. */
+dnb_status dnb_connected_act_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const float *biases,
+                                     const void *residual, int64_t ldr, void *y, int64_t ldy, int dtype,
+                                     int64_t batch, int64_t inputs, int64_t outputs, int act, void *workspace,
+                                     size_t workspace_bytes, dnb_stream stream);
+dnb_status dnb_connected_act_forward_workspace(const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
+                                               int64_t batch, int64_t inputs, int64_t outputs, size_t *bytes);
+/* Backward of dnb_connected_act_forward (connected.zig:121-138,170-200):
+ *   dz = delta * act'(y)                       out, rounded to dtype; also the residual's delta
+ *   dx (+)= dz * w                             added with DNB_ACC_DELTA
+ *   weight_updates (+)= dz^T * x               added with DNB_ACC_UPDATES
+ *   bias_updates (+)= sum over rows of dz      (from unrounded dz)
+ * The products take the rounded dz. y [batch][outputs] is the forward's output. With act linear, y is not
+ * read and dz is not written (dz = delta): both may be NULL. dz may be delta. dx, weight_updates and
+ * bias_updates may each be NULL: not computed. weight_updates [outputs][inputs] with row stride lddw is of
+ * updates_dtype: dtype, or DNB_F32 (for dnb_sgd_momentum). */
+dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *y,
+                                      int64_t ldy, const void *delta, int64_t ldd, void *dz, int64_t lddz, void *dx,
+                                      int64_t lddx, float *bias_updates, void *weight_updates, int64_t lddw,
+                                      int updates_dtype, int dtype, int64_t batch, int64_t inputs, int64_t outputs,
+                                      int act, int accumulate, void *workspace, size_t workspace_bytes,
+                                      dnb_stream stream);
+dnb_status dnb_connected_act_backward_workspace(const void *x, int64_t ldx, const void *w, int64_t ldw,
+                                                const void *delta, int64_t ldd, const void *dz, int64_t lddz,
+                                                int dtype, int64_t batch, int64_t inputs, int64_t outputs, int act,
+                                                size_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif

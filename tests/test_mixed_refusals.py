@@ -78,3 +78,39 @@ def test_sgd_refuses(built_lib, kw):
 
 def test_sgd_of_nothing(built_lib):
     assert sgd(rows=0) == 0 and sgd(cols=0, w=None) == 0
+
+
+def conn_fwd(x=P, ldx=16, w=2 * P, ldw=16, b=3 * P, r=4 * P, ldr=8, y=5 * P, ldy=8, dtype=BF16, M=4, K=16, N=8, act=7,
+             ws=None, wn=0):
+    return status("connected_act_forward", x, ldx, w, ldw, b, r, ldr, y, ldy, dtype, M, K, N, act, ws, wn, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=F32), dict(dtype=7), dict(M=-1), dict(K=-1), dict(N=-1), dict(act=14), dict(x=None), dict(w=None),
+    dict(y=None), dict(ldx=15), dict(ldw=15), dict(ldr=7), dict(ldy=7), dict(x=P + 1), dict(b=3 * P + 2), dict(y=P),
+    dict(y=2 * P + 32), dict(y=3 * P), dict(y=4 * P, ldy=9), dict(y=4 * P + 16), dict(ldx=1 << 62),
+    dict(M=100, x=P + 2, y=6 * P, ws=None), dict(M=100, ldx=17, y=6 * P, ws=7 * P, wn=10),
+])
+def test_connected_forward_refuses(built_lib, kw):
+    assert conn_fwd(**kw) == INVALID
+
+
+def test_connected_size_limits(built_lib):
+    assert conn_fwd(M=1 << 31) == UNSUPPORTED
+    assert conn_fwd(M=0, x=None, y=None) == 0 and conn_fwd(N=0, w=None) == 0
+
+
+def conn_bwd(x=P, ldx=16, w=2 * P, ldw=16, y=3 * P, ldy=8, d=4 * P, ldd=8, dz=5 * P, lddz=8, dx=6 * P, lddx=16, bu=7 * P,
+             wu=8 * P, lddw=16, ut=F32, dtype=BF16, M=4, K=16, N=8, act=7, acc=0, ws=9 * P, wn=1 << 19):
+    return status("connected_act_backward", x, ldx, w, ldw, y, ldy, d, ldd, dz, lddz, dx, lddx, bu, wu, lddw, ut, dtype,
+                  M, K, N, act, acc, ws, wn, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=F32), dict(ut=F16), dict(ut=9), dict(M=-1), dict(act=99), dict(acc=4), dict(x=None), dict(w=None),
+    dict(y=None), dict(d=None), dict(dz=None), dict(ldx=3), dict(ldd=7), dict(lddz=7), dict(lddx=15), dict(lddw=15),
+    dict(wu=8 * P + 2), dict(bu=7 * P + 1), dict(dx=P), dict(dx=4 * P), dict(wu=2 * P), dict(dz=4 * P, lddz=9),
+    dict(dz=3 * P), dict(bu=8 * P), dict(dx=5 * P), dict(ws=None), dict(wn=16), dict(ws=9 * P + 8),
+])
+def test_connected_backward_refuses(built_lib, kw):
+    assert conn_bwd(**kw) == INVALID
