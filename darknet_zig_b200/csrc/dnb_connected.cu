@@ -129,69 +129,7 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
         for (int j = 0; j < N; ++j) a.part[(int64_t)blockIdx.y * a.n + c + j] = sum[j];
 }
 
-// Adds the chunks' column sums in fp64, 8 slices of them in order, then the slices.
-__global__ void __launch_bounds__(256) k_column_sums(const float *part, int64_t chunks, int64_t n, float *out, int add) {
-    __shared__ double red[8][32];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
-    double s = 0.0;
-    if (c < n)
-#pragma unroll 4
-        for (int64_t q = ty; q < chunks; q += 8) s += (double)part[q * n + c];
-    red[ty][tx] = s;
-    __syncthreads();
-    if (ty == 0 && c < n) {
-        for (int i = 1; i < 8; ++i) s += red[i][tx];
-        out[c] = (float)(add ? (double)out[c] + s : s);
-    }
-}
-
 constexpr int kDzRows = 64;
-
-// ---- shared ----
-
-// Fills a matrix's rows with zeros (a product over nothing).
-__global__ void __launch_bounds__(256) k_zero_rows(unsigned char *p, int64_t rows, int64_t row_bytes, int64_t stride) {
-    const int64_t total = rows * row_bytes;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / row_bytes;
-        p[r * stride + (i - r * row_bytes)] = 0;
-    }
-}
-dnb_status zero_rows(void *p, int64_t rows, int64_t cols, int64_t ld, int64_t e, const DeviceState *ds, cudaStream_t s,
-                     const char *what) {
-    k_zero_rows<<<grid_for(rows * cols * e, 256, ds), 256, 0, s>>>(static_cast<unsigned char *>(p), rows, cols * e, ld * e);
-    return after_launch(s, what);
-}
-
-EpiOut epilogue(void *out, int64_t ld, int type, int64_t m, int64_t n) {
-    EpiOut e;
-    e.out = out;
-    e.ld = ld;
-    e.out_type = type;
-    e.m = m;
-    e.n = n;
-    e.vec_out = aligned16(out) && ld * dtype_size(type) % 16 == 0;
-    return e;
-}
-void add_to(EpiOut &e, const void *add, int64_t ld) {
-    e.add = add;
-    e.ld_add = ld;
-    e.vec_add = aligned16(add) && ld * dtype_size(e.out_type) % 16 == 0;
-}
-
-// A pair's 256 x 256 tiles where they fill the GPU's 74 pairs; else single CTAs' 128 x 128 tiles.
-bool big_tiles(int64_t m, int64_t n, const DeviceState *ds) {
-    return ((m + 255) / 256) * ((n + 255) / 256) >= ds->sm_count / 2;
-}
-
-template <bool A_MN, bool B_MN>
-dnb_status product(const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k, const EpiOut &e,
-                   const DeviceState *ds, cudaStream_t s, const char *what) {
-    if (big_tiles(m, n, ds))
-        return launch_gemm<GemmCfg<2, 256, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what);
-    return launch_gemm<GemmCfg<1, 128, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what);
-}
 
 constexpr int64_t kFewRows = 4;
 
@@ -227,21 +165,6 @@ BwdSpace bwd_space(void *ws, const void *x, int64_t ldx, const void *w, int64_t 
     return b;
 }
 
-dnb_status shape_check(int dtype, int64_t m, int64_t k, int64_t n, const char *what) {
-    if (!valid_dtype16(dtype)) return fail(DNB_ERR_INVALID, "%s: dtype must be bf16 or f16", what);
-    if (m < 0 || k < 0 || n < 0) return fail(DNB_ERR_INVALID, "%s: negative size", what);
-    if (m > 0x7fffffffll || k > 0x7fffffffll || n > 0x7fffffffll)
-        return fail(DNB_ERR_UNSUPPORTED, "%s: a size beyond 2^31 - 1", what);
-    return DNB_OK;
-}
-
-dnb_status workspace_check(void *ws, size_t have, size_t need, const char *what) {
-    if (need && (!ws || have < need || !aligned16(ws)))
-        return fail(DNB_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what, need,
-                    ws ? have : (size_t)0);
-    return DNB_OK;
-}
-
 }  // namespace
 }  // namespace dnb
 
@@ -253,7 +176,7 @@ dnb_status dnb_connected_act_forward_workspace(const void *x, int64_t ldx, const
                                                int64_t batch, int64_t inputs, int64_t outputs, size_t *bytes) {
     const char *what = "connected_act_forward_workspace";
     if (!bytes) return fail(DNB_ERR_INVALID, "%s: bytes is null", what);
-    DNB_TRY(shape_check(dtype, batch, inputs, outputs, what));
+    DNB_TRY(product_shape_check(dtype, batch, inputs, outputs, what));
     *bytes = fwd_space(nullptr, x, ldx, w, ldw, batch, inputs, outputs).total;
     return DNB_OK;
 }
@@ -263,7 +186,7 @@ dnb_status dnb_connected_act_forward(const void *x, int64_t ldx, const void *w, 
                                      int64_t batch, int64_t inputs, int64_t outputs, int act, void *workspace,
                                      size_t workspace_bytes, dnb_stream stream) {
     const char *what = "connected_act_forward";
-    DNB_TRY(shape_check(dtype, batch, inputs, outputs, what));
+    DNB_TRY(product_shape_check(dtype, batch, inputs, outputs, what));
     if (!valid_act(act)) return fail(DNB_ERR_INVALID, "%s: unknown activation %d", what, act);
     if (batch == 0 || outputs == 0) return DNB_OK;
     if (!y || (inputs > 0 && (!x || !w))) return fail(DNB_ERR_INVALID, "%s: null pointer", what);
@@ -297,17 +220,17 @@ dnb_status dnb_connected_act_forward(const void *x, int64_t ldx, const void *w, 
     }
     Operand a{x, ldx}, b{w, ldw};
     if (f.x) {
-        DNB_TRY(pack_rows(x, ldx, f.x, batch, inputs, nullptr, 0, ds, s, what));
+        DNB_TRY(pack_rows(x, ldx, f.x, batch, inputs, dtype, {}, ds, s, what));
         a = {f.x, packed_ld(inputs)};
     }
     if (f.w) {
-        DNB_TRY(pack_rows(w, ldw, f.w, outputs, inputs, nullptr, 0, ds, s, what));
+        DNB_TRY(pack_rows(w, ldw, f.w, outputs, inputs, dtype, {}, ds, s, what));
         b = {f.w, packed_ld(inputs)};
     }
     EpiOut e = epilogue(y, ldy, dtype, batch, outputs);
     e.bias = biases;
     e.act = act;
-    if (residual) add_to(e, residual, ldr);
+    if (residual) add_to(e, residual, ldr, dtype);
     return product<false, false>(a, b, dtype, batch, outputs, inputs, e, ds, s, what);
 }
 
@@ -317,7 +240,7 @@ dnb_status dnb_connected_act_backward_workspace(const void *x, int64_t ldx, cons
                                                 size_t *bytes) {
     const char *what = "connected_act_backward_workspace";
     if (!bytes) return fail(DNB_ERR_INVALID, "%s: bytes is null", what);
-    DNB_TRY(shape_check(dtype, batch, inputs, outputs, what));
+    DNB_TRY(product_shape_check(dtype, batch, inputs, outputs, what));
     const bool linear = act == DNB_ACT_LINEAR;
     *bytes = bwd_space(nullptr, x, ldx, w, ldw, linear ? delta : dz, linear ? ldd : lddz, batch, inputs, outputs).total;
     return DNB_OK;
@@ -330,7 +253,7 @@ dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w,
                                       int act, int accumulate, void *workspace, size_t workspace_bytes,
                                       dnb_stream stream) {
     const char *what = "connected_act_backward";
-    DNB_TRY(shape_check(dtype, batch, inputs, outputs, what));
+    DNB_TRY(product_shape_check(dtype, batch, inputs, outputs, what));
     if (!valid_act(act)) return fail(DNB_ERR_INVALID, "%s: unknown activation %d", what, act);
     if (accumulate & ~(DNB_ACC_UPDATES | DNB_ACC_DELTA)) return fail(DNB_ERR_INVALID, "%s: unknown accumulate bits", what);
     if (weight_updates && updates_dtype != dtype && updates_dtype != DNB_F32)
@@ -417,8 +340,7 @@ dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w,
         });
         DNB_TRY(st);
         if (bias_updates) {
-            k_column_sums<<<(unsigned)((outputs + 31) / 32), 256, 0, s>>>(f.part, chunks, outputs, bias_updates, add_w);
-            DNB_TRY(after_launch(s, what));
+            DNB_TRY(column_sums(f.part, chunks, outputs, outputs, bias_updates, add_w, s, what));
         }
     }
     if (inputs == 0) return DNB_OK;
@@ -427,22 +349,22 @@ dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w,
     if (dx) {
         Operand b{w, ldw};
         if (f.w) {
-            DNB_TRY(pack_rows(w, ldw, f.w, outputs, inputs, nullptr, 0, ds, s, what));
+            DNB_TRY(pack_rows(w, ldw, f.w, outputs, inputs, dtype, {}, ds, s, what));
             b = {f.w, packed_ld(inputs)};
         }
         EpiOut e = epilogue(dx, lddx, dtype, batch, inputs);
-        if (add_x) add_to(e, dx, lddx);
+        if (add_x) add_to(e, dx, lddx, dtype);
         const dnb_status st = product<false, true>(d, b, dtype, batch, inputs, outputs, e, ds, s, what);
         DNB_TRY(st);
     }
     if (weight_updates) {
         Operand b{x, ldx};
         if (f.x) {
-            DNB_TRY(pack_rows(x, ldx, f.x, batch, inputs, nullptr, 0, ds, s, what));
+            DNB_TRY(pack_rows(x, ldx, f.x, batch, inputs, dtype, {}, ds, s, what));
             b = {f.x, packed_ld(inputs)};
         }
         EpiOut e = epilogue(weight_updates, lddw, updates_dtype, outputs, inputs);
-        if (add_w) add_to(e, weight_updates, lddw);
+        if (add_w) add_to(e, weight_updates, lddw, updates_dtype);
         const dnb_status st = product<true, true>(d, b, dtype, outputs, inputs, batch, e, ds, s, what);
         DNB_TRY(st);
     }

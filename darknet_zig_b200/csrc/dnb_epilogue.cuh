@@ -5,22 +5,36 @@
 
 namespace dnb {
 
-// out = act(alpha * acc + bias[n] + add[m][n]), out and add of out_type (add may be out). A thread holds 32
-// columns of a row: 64 contiguous bytes of 16-bit output, 128 of fp32, so its accesses fill whole sectors.
+// out = act(f * acc + bias[n] + add[m][n]) (add may be out), f = alpha * *alpha_dev * row_factor[row].
+// With a row map, row r of the product is row rows[r] of out, add and row_factor. A thread holds 32 columns
+// of a row: 64 contiguous bytes of 16-bit output, 128 of fp32, so its accesses fill whole sectors.
 struct EpiOut {
     void *out = nullptr;
     int64_t ld = 0;
     int out_type = DNB_BF16;
+    int add_type = DNB_BF16;
     const void *add = nullptr;
     int64_t ld_add = 0;
     const float *bias = nullptr;
-    const float *alpha = nullptr;  // device scalar; NULL = 1
+    float alpha = 1.0f;
+    const float *alpha_dev = nullptr, *row_factor = nullptr;  // NULL = 1
+    const int *rows = nullptr, *m_dev = nullptr;
     int act = DNB_ACT_LINEAR;
     int64_t m = 0, n = 0;
     bool vec_out = false, vec_add = false;  // rows start on 16-byte boundaries
 
-    struct State {};
-    __device__ __forceinline__ void begin(State &, int64_t, int64_t) const {}
+    struct State {
+        int64_t row;  // of out; -1: none
+        float f;
+    };
+    __device__ __forceinline__ void begin(State &s, int64_t row, int64_t) const {
+        s.row = -1;
+        if (row >= (m_dev ? *m_dev : m)) return;
+        s.row = rows ? rows[row] : row;
+        s.f = alpha;
+        if (alpha_dev) s.f *= *alpha_dev;
+        if (row_factor) s.f *= row_factor[s.row];
+    }
     __device__ __forceinline__ void end(State &, int64_t, int64_t) const {}
 
     template <class T>
@@ -59,13 +73,13 @@ struct EpiOut {
                 if (j < cols) p[j] = Elem<T>::from(v[j]);
         }
     }
-    __device__ __forceinline__ void columns(State &, float (&v)[32], int64_t row, int64_t col) const {
-        if (row >= m) return;
+    __device__ __forceinline__ void columns(State &s, float (&v)[32], int64_t, int64_t col) const {
+        if (s.row < 0) return;
+        const int64_t row = s.row;
         const int cols = (int)(n - col < 32 ? n - col : 32);
-        if (alpha) {
-            const float a = *alpha;
+        if (s.f != 1.0f) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= a;
+            for (int j = 0; j < 32; ++j) v[j] *= s.f;
         }
         if (bias) {
 #pragma unroll
@@ -73,8 +87,8 @@ struct EpiOut {
                 if (j < cols) v[j] += __ldg(bias + col + j);
         }
         if (add) {
-            if (out_type == DNB_F32) load_add<float>(v, row, col, cols);
-            else if (out_type == DNB_BF16) load_add<__nv_bfloat16>(v, row, col, cols);
+            if (add_type == DNB_F32) load_add<float>(v, row, col, cols);
+            else if (add_type == DNB_BF16) load_add<__nv_bfloat16>(v, row, col, cols);
             else load_add<__half>(v, row, col, cols);
         }
         switch (act) {
@@ -103,5 +117,35 @@ struct EpiOut {
         for (int j = 0; j < 32; ++j) v[j] = activate_one(v[j], a);
     }
 };
+
+inline EpiOut epilogue(void *out, int64_t ld, int type, int64_t m, int64_t n) {
+    EpiOut e;
+    e.out = out;
+    e.ld = ld;
+    e.out_type = type;
+    e.m = m;
+    e.n = n;
+    e.vec_out = aligned16(out) && ld * dtype_size(type) % 16 == 0;
+    return e;
+}
+inline void add_to(EpiOut &e, const void *add, int64_t ld, int type) {
+    e.add = add;
+    e.ld_add = ld;
+    e.add_type = type;
+    e.vec_add = aligned16(add) && ld * dtype_size(type) % 16 == 0;
+}
+
+// A pair's 256 x 256 tiles where they fill a B200's 74 pairs and there is more than one CTA's tile of rows;
+// else single CTAs' 128 x 128 tiles. (Workspaces depend on it: a constant, not the current device's count.)
+inline bool big_tiles(int64_t m, int64_t n) { return m > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= 74; }
+
+template <bool A_MN, bool B_MN>
+dnb_status product(const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k, const EpiOut &e,
+                   const DeviceState *ds, cudaStream_t s, const char *what, const int *m_dev = nullptr,
+                   const int *k_dev = nullptr) {
+    if (big_tiles(m, n))
+        return launch_gemm<GemmCfg<2, 256, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
+    return launch_gemm<GemmCfg<1, 128, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
+}
 
 }  // namespace dnb

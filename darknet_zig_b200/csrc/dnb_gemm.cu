@@ -24,29 +24,69 @@ EncodeFn encoder() {
     return fn;
 }
 
-// Eight elements a thread: 16-byte stores whatever the source's alignment. Rows whose label is outside
-// [0, classes) become zeros and are not read.
-__global__ void __launch_bounds__(256) k_pack(const uint16_t *src, int64_t lds, uint16_t *dst, int64_t ldd,
-                                              int64_t rows, int64_t cols, int64_t per, const int32_t *labels,
-                                              int64_t classes) {
-    const int64_t total = rows * per;
+// Eight elements a thread: 16-byte stores whatever the source's alignment.
+template <class T>
+__global__ void __launch_bounds__(256) k_pack(const T *src, int64_t lds, T *dst, int64_t ldd, int64_t rows,
+                                              int64_t cols, int64_t per, Gather g) {
+    const int64_t kept = g.count ? *g.count : rows, end = g.count ? (kept + 63) / 64 * 64 : rows;
+    const int64_t total = end * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / per, c = (i - r * per) * 8;
-        const bool keep = !labels || (labels[r] >= 0 && labels[r] < classes);
-        uint16_t v[8] = {};
-        if (keep) {
-            const uint16_t *p = src + r * lds + c;
+        uint4 out = make_uint4(0u, 0u, 0u, 0u);
+        if (r < kept) {
+            const int64_t at = g.rows ? g.rows[r] : r;
+            const T *p = src + at * lds + c;
+            typename Vec<T, 16>::U u;
+            u.raw = out;
             if (c + 8 <= cols && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-                *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
+                u.raw = *reinterpret_cast<const uint4 *>(p);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (c + j < cols) v[j] = p[j];
+                    if (c + j < cols) u.e[j] = p[j];
             }
+            if (g.factor) {
+                float f[8];
+                Vec<T, 16>::unpack(u.raw, f);
+                const float by = g.factor[at] * *g.norm;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] *= by;
+                u.raw = Vec<T, 16>::pack(f);
+            }
+            out = u.raw;
         }
-        *reinterpret_cast<uint4 *>(dst + r * ldd + c) =
-            make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16,
-                       v[6] | (uint32_t)v[7] << 16);
+        *reinterpret_cast<uint4 *>(dst + r * ldd + c) = out;
+    }
+}
+
+// Adds the chunks' column sums in fp64, 8 slices of them in order, then the slices.
+__global__ void __launch_bounds__(256) k_column_sums(const float *part, int64_t chunks, int64_t n, int64_t ld,
+                                                     float *out, int add) {
+    __shared__ double red[8][32];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+    double s = 0.0;
+    if (c < n)
+#pragma unroll 4
+        for (int64_t q = ty; q < chunks; q += 8) s += (double)part[q * ld + c];
+    red[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < n) {
+        for (int i = 1; i < 8; ++i) s += red[i][tx];
+        out[c] = (float)(add ? (double)out[c] + s : s);
+    }
+}
+
+// A block per row; 16-byte stores where every row starts on that boundary, else 2-byte ones.
+__global__ void __launch_bounds__(256) k_zero_rows(unsigned char *p, int64_t rows, int64_t row_bytes, int64_t stride,
+                                                   const int32_t *labels, int64_t classes, bool wide) {
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        if (labels && labels[r] >= 0 && labels[r] < classes) continue;
+        unsigned char *q = p + r * stride;
+        const int64_t head = wide ? row_bytes / 16 * 16 : 0;
+        for (int64_t i = threadIdx.x * 16; i < head; i += 256 * 16)
+            *reinterpret_cast<uint4 *>(q + i) = make_uint4(0u, 0u, 0u, 0u);
+        for (int64_t i = head + threadIdx.x * 2; i < row_bytes; i += 256 * 2) *reinterpret_cast<uint16_t *>(q + i) = 0;
     }
 }
 
@@ -71,12 +111,27 @@ dnb_status make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t oute
     return DNB_OK;
 }
 
-dnb_status pack_rows(const void *src, int64_t lds, void *dst, int64_t rows, int64_t cols, const int32_t *labels,
-                     int64_t classes, const DeviceState *ds, cudaStream_t s, const char *what) {
-    const int64_t per = (cols + 7) / 8;
-    k_pack<<<grid_for(rows * per, 256, ds), 256, 0, s>>>(static_cast<const uint16_t *>(src), lds,
-                                                         static_cast<uint16_t *>(dst), packed_ld(cols), rows, cols,
-                                                         per, labels, classes);
+dnb_status pack_rows(const void *src, int64_t lds, void *dst, int64_t rows, int64_t cols, int dtype, const Gather &g,
+                     const DeviceState *ds, cudaStream_t s, const char *what) {
+    const int64_t per = (cols + 7) / 8, out_rows = g.count ? (rows + 63) / 64 * 64 : rows;
+    return dispatch_dtype16(dtype, [&]<class T>() {
+        k_pack<T><<<grid_for(out_rows * per, 256, ds), 256, 0, s>>>(static_cast<const T *>(src), lds,
+                                                                    static_cast<T *>(dst), packed_ld(cols), rows, cols,
+                                                                    per, g);
+        return after_launch(s, what);
+    });
+}
+
+dnb_status column_sums(const float *part, int64_t chunks, int64_t n, int64_t ld, float *out, bool add, cudaStream_t s,
+                       const char *what) {
+    k_column_sums<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(part, chunks, n, ld, out, add);
+    return after_launch(s, what);
+}
+
+dnb_status zero_rows(void *p, int64_t rows, int64_t cols, int64_t ld, int64_t e, const DeviceState *ds, cudaStream_t s,
+                     const char *what, const int32_t *labels, int64_t classes) {
+    k_zero_rows<<<grid_for(rows, 1, ds), 256, 0, s>>>(static_cast<unsigned char *>(p), rows, cols * e, ld * e, labels,
+                                                      classes, aligned16(p) && ld * e % 16 == 0);
     return after_launch(s, what);
 }
 

@@ -47,6 +47,7 @@ struct GemmArgs {
     int m_tiles, n_tiles, k_blocks;
     int band;       // output tiles are taken in bands of this many row tiles, down the rows first
     unsigned idesc; // the tensor core's instruction descriptor
+    const int *m_dev, *k_dev;  // the rows / the reduction's length where the device knows them (NULL: as above)
     unsigned long long wait_ns;
     unsigned *error_word;
 };
@@ -218,9 +219,9 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
 }
 
 // The row tile and column tile of the t-th tile.
-__device__ __forceinline__ void tile_at(const GemmArgs &g, int t, int &mt, int &nt) {
+__device__ __forceinline__ void tile_at(const GemmArgs &g, int m_tiles, int t, int &mt, int &nt) {
     const int per = g.band * g.n_tiles, b = t / per, in = t - b * per;
-    const int rows = min(g.band, g.m_tiles - b * g.band);
+    const int rows = min(g.band, m_tiles - b * g.band);
     nt = in / rows;
     mt = b * g.band + (in - nt * rows);
 }
@@ -270,7 +271,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if constexpr (CTAS == 2) cluster_sync();
     fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int tiles = g.m_tiles * g.n_tiles, step = (int)gridDim.x / CTAS, first = (int)blockIdx.x / CTAS;
+    const int m_tiles = g.m_dev ? (*g.m_dev + C::TM - 1) / C::TM : g.m_tiles;
+    const int k_blocks = g.k_dev ? (*g.k_dev + kBlockK - 1) / kBlockK : g.k_blocks;
+    const int tiles = m_tiles * g.n_tiles, step = (int)gridDim.x / CTAS, first = (int)blockIdx.x / CTAS;
 
     if (warp == 0 && lane == 0) {
         // loads
@@ -278,9 +281,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         bool ok = true;
         for (int t = first; ok && t < tiles; t += step) {
             int mt, nt;
-            tile_at(g, t, mt, nt);
+            tile_at(g, m_tiles, t, mt, nt);
             const int am = mt * C::TM + (int)rank * C::BM, bn = nt * C::BN + (int)rank * C::BROWS;
-            for (int kb = 0; kb < g.k_blocks; ++kb, ++it) {
+            for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                 const int s = it % S;
                 if (!mbar_wait(empty + 8 * s, ((it / S) & 1) ^ 1, g, gave_up)) {
                     ok = false;
@@ -321,7 +324,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             if (!mbar_wait(acc_empty + 8 * b, ((n >> 1) & 1) ^ 1, g, gave_up)) break;
             fence_after();
             const uint32_t d = tmem + b * C::BN;
-            for (int kb = 0; kb < g.k_blocks; ++kb, ++it) {
+            for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                 const int s = it % S;
                 if (!mbar_wait(full + 8 * s, (it / S) & 1, g, gave_up)) {
                     ok = false;
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         for (int t = first; t < tiles; t += step, ++n) {
             const int b = n & 1;
             int mt, nt;
-            tile_at(g, t, mt, nt);
+            tile_at(g, m_tiles, t, mt, nt);
             const bool ok = mbar_wait(acc_full + 8 * b, (n >> 1) & 1, g, gave_up);
             if (!__all_sync(0xffffffffu, ok)) break;
             fence_after();
@@ -357,7 +360,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             for (int c = 0; c < C::BN; c += 32) {
                 if (col0 + c >= g.n) break;
                 float v[32];
-                tmem_load32(at + c, v);
+                if (k_blocks > 0) {
+                    tmem_load32(at + c, v);
+                } else {  // a sum over nothing
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                }
                 epi.columns(st, v, row, col0 + c);
             }
             fence_before();
@@ -374,10 +382,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (warp == 2) tmem_free<CTAS>(tmem, C::TMEM_COLS);
 }
 
-// Launches the product of a and b (already TMA-ready).
+// Launches the product of a and b (already TMA-ready). With m_dev / k_dev, m and k are what they may reach.
 template <class C, class Epi>
 dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k, const Epi &epi,
-                       const DeviceState *ds, cudaStream_t s, const char *what) {
+                       const DeviceState *ds, cudaStream_t s, const char *what, const int *m_dev = nullptr,
+                       const int *k_dev = nullptr) {
     static std::atomic<int> opted[kMaxDevices];
     auto kernel = k_gemm<C, Epi>;
     if (!opted[ds->device].load(std::memory_order_acquire)) {
@@ -399,6 +408,8 @@ dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m,
     g.n_tiles = (int)nt;
     g.k_blocks = (int)((k + kBlockK - 1) / kBlockK);
     g.band = 8;
+    g.m_dev = m_dev;
+    g.k_dev = k_dev;
     // fp32 accumulators; operand type; majors; n / 8; m / 16
     const unsigned t = dtype == DNB_BF16 ? 1u : 0u;
     g.idesc = (1u << 4) | (t << 7) | (t << 10) | ((C::A_MN ? 1u : 0u) << 15) | ((C::B_MN ? 1u : 0u) << 16) |

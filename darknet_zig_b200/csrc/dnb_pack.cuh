@@ -8,10 +8,37 @@ namespace dnb {
 inline int64_t packed_ld(int64_t cols) { return (cols + 7) / 8 * 8; }
 inline int64_t packed_bytes(int64_t rows, int64_t cols) { return rows * packed_ld(cols) * 2; }
 
-// Copies a matrix to rows packed_ld(cols) apart at a 16-byte aligned dst; with labels, rows whose label is
-// outside [0, classes) become zeros without being read. dnb_gemm.cu.
-dnb_status pack_rows(const void *src, int64_t lds, void *dst, int64_t rows, int64_t cols, const int32_t *labels,
-                     int64_t classes, const DeviceState *ds, cudaStream_t s, const char *what);
+// Copies a matrix to rows packed_ld(cols) apart at a 16-byte aligned dst. With a row map, the map's first
+// *count rows are gathered, and zero rows follow up to a multiple of 64. With factors, row r of the source is
+// multiplied by factor[r] * *norm and rounded again. dnb_gemm.cu.
+struct Gather {
+    const int *rows = nullptr, *count = nullptr;
+    const float *factor = nullptr, *norm = nullptr;
+};
+dnb_status pack_rows(const void *src, int64_t lds, void *dst, int64_t rows, int64_t cols, int dtype, const Gather &g,
+                     const DeviceState *ds, cudaStream_t s, const char *what);
+
+inline dnb_status product_shape_check(int dtype, int64_t m, int64_t k, int64_t n, const char *what) {
+    if (!valid_dtype16(dtype)) return fail(DNB_ERR_INVALID, "%s: dtype must be bf16 or f16", what);
+    if (m < 0 || k < 0 || n < 0) return fail(DNB_ERR_INVALID, "%s: negative size", what);
+    if (m > 0x7fffffffll || k > 0x7fffffffll || n > 0x7fffffffll)
+        return fail(DNB_ERR_UNSUPPORTED, "%s: a size beyond 2^31 - 1", what);
+    return DNB_OK;
+}
+
+inline dnb_status workspace_check(void *ws, size_t have, size_t need, const char *what) {
+    if (need && (!ws || have < need || !aligned16(ws)))
+        return fail(DNB_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what, need,
+                    ws ? have : (size_t)0);
+    return DNB_OK;
+}
+
+// out[c] (+)= the sum of part[q][c] over the chunks q, rows of `part` ld apart; in fp64, in a fixed order.
+dnb_status column_sums(const float *part, int64_t chunks, int64_t n, int64_t ld, float *out, bool add, cudaStream_t s,
+                       const char *what);
+// Fills a matrix's rows with zeros; with labels, only the rows whose label is outside [0, classes).
+dnb_status zero_rows(void *p, int64_t rows, int64_t cols, int64_t ld, int64_t e, const DeviceState *ds, cudaStream_t s,
+                     const char *what, const int32_t *labels = nullptr, int64_t classes = 0);
 
 // Hands out 256-byte aligned pieces of a workspace (of nothing: only their sum).
 struct Carver {

@@ -405,6 +405,38 @@ def connectedActBackward(x, w, y, delta, dz, dx, bias_updates, weight_updates, b
          accumulate, ws, wn, _s())
 
 
+def connectedXentForward(x, w, biases, labels, loss, lse, batch, inputs, classes, workspace=None):  # noqa: N802
+    """Per row: lse = log sum exp of x w^T + biases, loss = lse minus the label's output, without storing the
+    outputs. labels int32; a row whose label is outside [0, classes) is padding (loss and lse 0)."""
+    dt = _dtype(x, "x")
+    px, ldx = _mat(x, "x", batch, inputs, x.dtype)
+    pw, ldw = _mat(w, "w", classes, inputs, x.dtype)
+    ws, wn, _keep = _workspace(workspace, "connected_xent_forward_workspace", _align(px), ldx, _align(pw), ldw, dt,
+                               batch, inputs, classes)
+    call("connected_xent_forward", px, ldx, pw, ldw, _vec(biases, "biases", classes, optional=True),
+         _vec(labels, "labels", batch, torch.int32), _vec(loss, "loss", batch), _vec(lse, "lse", batch), dt, batch,
+         inputs, classes, ws, wn, _s())
+
+
+def connectedXentBackward(x, w, biases, labels, lse, row_scales, scale, dx, bias_updates,  # noqa: N802
+                          weight_updates, batch, inputs, classes, accumulate=ACC_UPDATES, workspace=None):
+    """Deltas of connectedXentForward in darknet's sign, times scale and each row's row_scales (None: 1). dx,
+    bias_updates (fp32) and weight_updates (x's type or fp32) may each be None; see connectedActBackward for
+    accumulate."""
+    dt = _dtype(x, "x")
+    px, ldx = _mat(x, "x", batch, inputs, x.dtype)
+    pw, ldw = _mat(w, "w", classes, inputs, x.dtype)
+    pdx, lddx = _mat(dx, "dx", batch, inputs, x.dtype, optional=True)
+    pu, ldu, ut = _updates(weight_updates, classes, inputs, x.dtype)
+    ws, wn, _keep = _workspace(workspace, "connected_xent_backward_workspace", _align(px), ldx, _align(pw), ldw, dt,
+                               batch, inputs, classes)
+    call("connected_xent_backward", px, ldx, pw, ldw, _vec(biases, "biases", classes, optional=True),
+         _vec(labels, "labels", batch, torch.int32), _vec(lse, "lse", batch),
+         _vec(row_scales, "row_scales", batch, optional=True), scale, pdx, lddx,
+         _vec(bias_updates, "bias_updates", classes, optional=True), pu, ldu, ut, dt, batch, inputs, classes,
+         accumulate, ws, wn, _s())
+
+
 def _updates(t, rows, cols, dtype):
     """(pointer, row stride, type) of weight updates: the operands' type or fp32."""
     if t is None:

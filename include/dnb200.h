@@ -479,6 +479,38 @@ dnb_status dnb_connected_act_backward_workspace(const void *x, int64_t ldx, cons
                                                 int dtype, int64_t batch, int64_t inputs, int64_t outputs, int act,
                                                 size_t *bytes);
 
+/* Softmax + cross entropy of a connected layer's outputs (dnb_softmax_xent after the connected layer)
+ * without storing them: z[m][n] = sum_k x[m][k] * w[n][k] + biases[n] is formed tile by tile;
+ *   lse[m] = log(sum_n exp(z[m][n]));  loss[m] = lse[m] - z[m][labels[m]].
+ * x [batch][inputs], w [classes][inputs] of dtype (bf16 or f16), inputs and classes positive; biases may be
+ * NULL. labels int32: a row
+ * whose label is not in [0, classes) is padding: its loss and lse are 0 and its x is never used (it may
+ * hold NaN). */
+dnb_status dnb_connected_xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const float *biases,
+                                      const int32_t *labels, float *loss, float *lse, int dtype, int64_t batch,
+                                      int64_t inputs, int64_t classes, void *workspace, size_t workspace_bytes,
+                                      dnb_stream stream);
+dnb_status dnb_connected_xent_forward_workspace(const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
+                                                int64_t batch, int64_t inputs, int64_t classes, size_t *bytes);
+/* Its deltas, with the reference's sign (truth - prediction, blas.zig:251: minus the loss's gradient, so
+ * that the updates are added to the weights):
+ *   d[m][n] = scale * row_scales[m] * ((n == labels[m]) - exp(z[m][n] - lse[m])), 0 in a padding row;
+ *   dx (+)= d * w;  weight_updates (+)= d^T * x;  bias_updates (+)= sum over rows of d
+ * (added with DNB_ACC_DELTA / DNB_ACC_UPDATES). lse is the forward's. row_scales may be NULL (1). dx,
+ * weight_updates and bias_updates may each be NULL. d is formed for a piece of the classes at a time; the
+ * products take d / (scale * row_scales[m]) rounded to dtype (times 2^14, so that f16 keeps small
+ * probabilities) and multiply by the factors afterwards; with row_scales, weight_updates takes x times its
+ * row's factor, rounded to dtype. bias_updates takes d unrounded. dx of a padding row is 0 (unchanged when
+ * added to). */
+dnb_status dnb_connected_xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, const float *biases,
+                                       const int32_t *labels, const float *lse, const float *row_scales, float scale,
+                                       void *dx, int64_t lddx, float *bias_updates, void *weight_updates,
+                                       int64_t lddw, int updates_dtype, int dtype, int64_t batch, int64_t inputs,
+                                       int64_t classes, int accumulate, void *workspace, size_t workspace_bytes,
+                                       dnb_stream stream);
+dnb_status dnb_connected_xent_backward_workspace(const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
+                                                 int64_t batch, int64_t inputs, int64_t classes, size_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -114,3 +114,33 @@ def conn_bwd(x=P, ldx=16, w=2 * P, ldw=16, y=3 * P, ldy=8, d=4 * P, ldd=8, dz=5 
 ])
 def test_connected_backward_refuses(built_lib, kw):
     assert conn_bwd(**kw) == INVALID
+
+
+def xent_fwd(x=P, ldx=16, w=2 * P, ldw=16, b=3 * P, lab=4 * P, loss=5 * P, lse=6 * P, dtype=BF16, M=4, K=16, N=8,
+             ws=7 * P, wn=1 << 19):
+    return status("connected_xent_forward", x, ldx, w, ldw, b, lab, loss, lse, dtype, M, K, N, ws, wn, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=F32), dict(M=-1), dict(K=0), dict(N=0), dict(x=None), dict(w=None), dict(lab=None), dict(loss=None),
+    dict(lse=None), dict(ldx=15), dict(ldw=1), dict(x=P + 1), dict(lab=4 * P + 2), dict(loss=5 * P + 1),
+    dict(lse=5 * P), dict(loss=P), dict(lse=4 * P), dict(ws=None), dict(wn=8), dict(ws=7 * P + 4),
+])
+def test_xent_forward_refuses(built_lib, kw):
+    assert xent_fwd(**kw) == INVALID
+
+
+def xent_bwd(x=P, ldx=16, w=2 * P, ldw=16, b=3 * P, lab=4 * P, lse=5 * P, rs=6 * P, dx=7 * P, lddx=16, bu=8 * P,
+             wu=9 * P, lddw=16, ut=F32, dtype=BF16, M=4, K=16, N=8, acc=0, ws=10 * P, wn=1 << 19):
+    return status("connected_xent_backward", x, ldx, w, ldw, b, lab, lse, rs, 1.0, dx, lddx, bu, wu, lddw, ut, dtype, M,
+                  K, N, acc, ws, wn, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=F32), dict(ut=F16), dict(M=-1), dict(K=0), dict(N=0), dict(acc=8), dict(x=None), dict(w=None),
+    dict(lab=None), dict(lse=None), dict(ldx=15), dict(ldw=15), dict(lddx=15), dict(lddw=15), dict(rs=6 * P + 2),
+    dict(dx=P), dict(wu=2 * P), dict(bu=3 * P), dict(wu=7 * P), dict(bu=5 * P), dict(ws=None), dict(wn=64),
+    dict(ws=10 * P + 8),
+])
+def test_xent_backward_refuses(built_lib, kw):
+    assert xent_bwd(**kw) == INVALID
