@@ -1,13 +1,15 @@
 // Group norm + activation on channels-last tensors, forward (the batchnorm layer's place,
 // batchnorm.zig:129-153, with statistics per image and group instead of per batch).
 //
-//   mean = sum(x)/n,  rstd = 1/sqrt(sum((x - mean)^2)/n + eps),  y = act(((x - mean)*rstd)*scale + bias)
+//   mean = sum(x)/n,  rstd = 1/sqrt(sum((x - mean)^2)/n + eps),  y = act((x - mean)*(rstd*scale) + bias)
 //
 // Bound by memory: x in, y out, nothing else of that size. k_gn_fwd reads a unit (see dnb_gn.cuh) once
-// into shared memory, adds it up on the way, takes the squared deviations from the true mean in a second
-// walk over shared memory (no cancellation, whatever the mean), and writes y in a third. Per-thread sums
-// run over a column's rows / RL elements in fp32; they are added across threads and CTAs in fp64, in a
-// fixed order.
+// into shared memory and adds it up on the way; y comes from shared memory. The sums are of d = x - s and
+// d^2 about a shift s of each thread's own, the first element it sees of the group: s is one of the group's
+// elements, so s's own distance from the mean is among the deviations that make up the variance, and no mean,
+// however far from 0, cancels. Each thread's (count, mean, squared deviations) are merged in fp64 (Chan,
+// Golub and LeVeque), in a fixed order. With a second walk over shared memory for the deviations instead,
+// [128,784,256] bf16 took 45 us, bound by instructions (30 an element against 9 now).
 #include "dnb_gn.cuh"
 
 namespace dnb {
@@ -18,168 +20,212 @@ struct GnFwd {
     void *y;
     const float *scales, *biases;
     float *mean, *rstd;
-    double *pieces;  // streaming path: [batch][groups][chunks][2] = (mean, M2) of a row chunk
+    double2 *pieces;  // streaming path: [batch][groups][chunks] = (mean, M2) of a row chunk
     int64_t spatial, filters, groups, cg, cb, nu, rows, chunks;
     float eps;
     int act, cluster;
-    unsigned slab, part;  // bytes, floats
+    unsigned slab, part;  // bytes, entries
 };
 
-// Adds part[rl][c] over rl and the channels of each group: a warp per group, fp64.
-__device__ __forceinline__ void group_sums(const float *part, int rl_n, int cb, int ng, int cg, double *out) {
-    const int lane = threadIdx.x & 31;
-    for (int g = threadIdx.x >> 5; g < ng; g += blockDim.x >> 5) {
-        double s = 0.0;
-        if (cg >= 32) {
-            for (int r = 0; r < rl_n; ++r)
-                for (int c = lane; c < cg; c += 32) s += (double)part[r * cb + g * cg + c];
-        } else {  // several rows at a time
-            const int per = 32 / cg, r0 = lane / cg, c = lane % cg;
-            if (r0 < per)
-                for (int r = r0; r < rl_n; r += per) s += (double)part[r * cb + g * cg + c];
+// Merges the moments of a group's threads: entries (rl, e) with e < eg of the group, each `per` elements of a
+// row times the thread's rows. A warp's lanes all get (mean, M2).
+__device__ __forceinline__ double2 merge_group(const float *mean, const float *m2, int rl_n, int pitch, int e0, int eg,
+                                               int per, int nr) {
+    const int lane = threadIdx.x & 31, total = rl_n * eg;
+    const int step_r = 32 / eg, step_e = 32 - step_r * eg;
+    double n = 0.0, s = 0.0;
+    int r = lane / eg, e = lane - r * eg;
+    for (int i = lane; i < total; i += 32) {
+        const int rows = nr > r ? (nr - r + rl_n - 1) / rl_n : 0;
+        const double w = (double)(rows * per);
+        if (rows) {
+            n += w;
+            s += w * (double)mean[r * pitch + e0 + e];
         }
-        s = warp_sum(s);
-        if (lane == 0) out[g] = s;
+        r += step_r;
+        e += step_e;
+        if (e >= eg) {
+            e -= eg;
+            ++r;
+        }
     }
+    n = warp_sum(n);
+    s = warp_sum(s);
+    const double mu = n > 0.0 ? s / n : 0.0;
+    double q = 0.0;
+    r = lane / eg;
+    e = lane - r * eg;
+    for (int i = lane; i < total; i += 32) {
+        const int rows = nr > r ? (nr - r + rl_n - 1) / rl_n : 0;
+        if (rows) {
+            const double d = (double)mean[r * pitch + e0 + e] - mu;
+            q += (double)m2[r * pitch + e0 + e] + (double)(rows * per) * d * d;
+        }
+        r += step_r;
+        e += step_e;
+        if (e >= eg) {
+            e -= eg;
+            ++r;
+        }
+    }
+    return make_double2(mu, warp_sum(q));
 }
 
-template <class T, int VB, int A, bool STREAM>
+template <class T, int VB, int A, bool UNI, bool STREAM>
 __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a) {
-    using V = Vec<T, VB>;
+    using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
-    constexpr int N = V::N;
+    constexpr int N = V::N, P = V::P;
     extern __shared__ __align__(16) unsigned char smem[];
     const Place p = place_of(a, STREAM ? a.chunks : a.cluster);
     T *slab = reinterpret_cast<T *>(smem);
-    float *part = reinterpret_cast<float *>(smem + a.slab);
-    double *gs = reinterpret_cast<double *>(smem + ((a.slab + a.part * 4 + 15) & ~15u));  // [2][ng] sums
-    float *gm = reinterpret_cast<float *>(gs + 2 * p.ng), *gr = gm + p.ng;               // mean, rstd
+    float *pm = reinterpret_cast<float *>(smem + a.slab), *pq = pm + a.part;  // the threads' means and M2
+    double2 *gs = reinterpret_cast<double2 *>(smem + ((a.slab + a.part * 8 + 15) & ~15u));  // the CTA's, a group
+    float *gm = reinterpret_cast<float *>(gs + p.ng), *gr = gm + p.ng;                       // mean, rstd
     const int nt = blockDim.x, v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
     const bool on = rl < rl_n;
     const T *x = static_cast<const T *>(a.x) + (p.b * a.spatial + p.r0) * a.filters + p.c0;
     const int cg = (int)a.cg;
-    const double count = STREAM ? (double)p.nr * (double)a.cg : (double)a.spatial * (double)a.cg;
+    const int64_t pitch = a.filters * rl_n;
 
-    // load, keep, and add up
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
-        float acc[N] = {};
-        const T *src = x + (int64_t)col * N;
-        T *dst = slab + col * N;
-        int r = rl;
+        float2 s1[P] = {}, s2[P] = {}, sh[P] = {};
+        const T *src = x + (int64_t)rl * a.filters + (int64_t)col * N;
+        T *dst = slab + rl * p.cb + col * N;
+        const int rows = p.nr > rl ? (p.nr - rl + rl_n - 1) / rl_n : 0;
+        if (rows) {
+            V::unpack(*reinterpret_cast<const Raw *>(src), sh);
+            if constexpr (UNI) {
+#pragma unroll
+                for (int i = P - 1; i >= 0; --i) sh[i] = both(sh[0].x);
+            }
+        }
         constexpr int U = 4;
-        for (; r + (U - 1) * rl_n < p.nr; r += U * rl_n) {
+        int r = 0;
+        for (; r + U <= rows; r += U) {
             Raw raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                raw[u] = *reinterpret_cast<const Raw *>(src + (int64_t)(r + u * rl_n) * a.filters);
+            for (int u = 0; u < U; ++u) raw[u] = *reinterpret_cast<const Raw *>(src + u * pitch);
+            src += U * pitch;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float f[N];
+                float2 f[P];
                 V::unpack(raw[u], f);
-                *reinterpret_cast<Raw *>(dst + (r + u * rl_n) * p.cb) = raw[u];
+                if constexpr (!STREAM) *reinterpret_cast<Raw *>(dst + u * rl_n * p.cb) = raw[u];
 #pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] += f[j];
+                for (int i = 0; i < P; ++i) {
+                    const float2 d = __fadd2_rn(f[i], neg(sh[i]));
+                    s1[i] = __fadd2_rn(s1[i], d);
+                    s2[i] = __ffma2_rn(d, d, s2[i]);
+                }
+            }
+            dst += U * rl_n * p.cb;
+        }
+        for (; r < rows; ++r) {
+            const Raw raw = *reinterpret_cast<const Raw *>(src);
+            src += pitch;
+            float2 f[P];
+            V::unpack(raw, f);
+            if constexpr (!STREAM) *reinterpret_cast<Raw *>(dst) = raw;
+            dst += rl_n * p.cb;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const float2 d = __fadd2_rn(f[i], neg(sh[i]));
+                s1[i] = __fadd2_rn(s1[i], d);
+                s2[i] = __ffma2_rn(d, d, s2[i]);
             }
         }
-        for (; r < p.nr; r += rl_n) {
-            const Raw raw = *reinterpret_cast<const Raw *>(src + (int64_t)r * a.filters);
-            float f[N];
-            V::unpack(raw, f);
-            *reinterpret_cast<Raw *>(dst + r * p.cb) = raw;
+        // (mean, M2) about the thread's own mean: M2 = sum d^2 - (sum d)^2 / count
+        if constexpr (UNI) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] += f[j];
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) part[rl * p.cb + col * N + j] = acc[j];
-    }
-    __syncthreads();
-    group_sums(part, rl_n, p.cb, p.ng, cg, gs);
-    const int q_n = STREAM ? 1 : a.cluster;
-    if (q_n > 1) gn_cluster_sync();
-    else __syncthreads();
-    for (int g = threadIdx.x; g < p.ng; g += nt) {
-        double s = 0.0;
-        if (q_n > 1)
-            for (int q = 0; q < q_n; ++q) s += gn_peer_f64(gs + g, (unsigned)q);
-        else
-            s = gs[g];
-        gm[g] = (float)(s / count);
-    }
-    __syncthreads();
-
-    // squared deviations, from shared memory
-    for (int col = col0; col < v; col += vp) {
-        if (!on) break;
-        float acc[N] = {}, m[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) m[j] = gm[(col * N + j) / cg];
-        for (int r = rl; r < p.nr; r += rl_n) {
-            float f[N];
-            V::unpack(*reinterpret_cast<const Raw *>(slab + r * p.cb + col * N), f);
+            for (int i = 1; i < P; ++i) {
+                s1[0] = __fadd2_rn(s1[0], s1[i]);
+                s2[0] = __fadd2_rn(s2[0], s2[i]);
+            }
+            const float t1 = N > 1 ? s1[0].x + s1[0].y : s1[0].x, t2 = N > 1 ? s2[0].x + s2[0].y : s2[0].x;
+            const float inv = rows ? __fdividef(1.0f, (float)(rows * N)) : 0.0f;
+            pm[rl * v + col] = __fmaf_rn(t1, inv, sh[0].x);
+            const float q = __fmaf_rn(-t1 * inv, t1, t2);
+            pq[rl * v + col] = q < 0.0f ? 0.0f : q;
+        } else {
+            const float inv = rows ? __fdividef(1.0f, (float)rows) : 0.0f;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float d = f[j] - m[j];
-                acc[j] = __fmaf_rn(d, d, acc[j]);
+                const float t1 = j & 1 ? s1[j / 2].y : s1[j / 2].x, t2 = j & 1 ? s2[j / 2].y : s2[j / 2].x;
+                const float q = __fmaf_rn(-t1 * inv, t1, t2);
+                pm[rl * p.cb + col * N + j] = __fmaf_rn(t1, inv, j & 1 ? sh[j / 2].y : sh[j / 2].x);
+                pq[rl * p.cb + col * N + j] = q < 0.0f ? 0.0f : q;
             }
         }
-#pragma unroll
-        for (int j = 0; j < N; ++j) part[rl * p.cb + col * N + j] = acc[j];
     }
     __syncthreads();
-    double *gv = gs + p.ng;
-    group_sums(part, rl_n, p.cb, p.ng, cg, gv);
-    if (q_n > 1) gn_cluster_sync();
-    else __syncthreads();
-    for (int g = threadIdx.x; g < p.ng; g += nt) {
-        double s = 0.0;
-        if (q_n > 1)
-            for (int q = 0; q < q_n; ++q) s += gn_peer_f64(gv + g, (unsigned)q);
-        else
-            s = gv[g];
+    const int eg = UNI ? cg / N : cg, lane = threadIdx.x & 31;
+    const int q_n = STREAM ? 1 : a.cluster;
+    for (int g = threadIdx.x >> 5; g < p.ng; g += nt >> 5) {
+        const double2 s = merge_group(pm, pq, rl_n, UNI ? v : p.cb, g * eg, eg, UNI ? N : 1, p.nr);
+        if (lane != 0) continue;
         if constexpr (STREAM) {
-            // the deviations are from the rounded mean: their sum is M2 + n (mean - gm)^2, taken back here
-            const double mean = gs[g] / count, e = mean - (double)gm[g];
-            double *piece = a.pieces + ((p.b * a.groups + p.g0 + g) * a.chunks + blockIdx.x % a.chunks) * 2;
-            const double m2 = s - count * e * e;
-            piece[0] = mean;
-            piece[1] = m2 < 0.0 ? 0.0 : m2;
+            a.pieces[(p.b * a.groups + p.g0 + g) * a.chunks + blockIdx.x % a.chunks] = s;
+        } else if (q_n == 1) {
+            gm[g] = (float)s.x;
+            gr[g] = (float)rsqrt(s.y / ((double)a.spatial * (double)cg) + (double)a.eps);
         } else {
-            const float rstd = (float)(1.0 / sqrt(s / count + (double)a.eps));
-            gr[g] = rstd;
-            if (p.r0 == 0) {  // the unit's first CTA
-                a.mean[p.b * a.groups + p.g0 + g] = gm[g];
-                a.rstd[p.b * a.groups + p.g0 + g] = rstd;
-            }
+            gs[g] = s;
         }
     }
     if constexpr (STREAM) return;
-    // the peers may still read gv: no CTA leaves before all have
-    if (q_n > 1) gn_cluster_sync();
-    else __syncthreads();
+    if (q_n > 1) {
+        gn_cluster_arrive();
+        gn_cluster_wait();
+        for (int g = threadIdx.x; g < p.ng; g += nt) {
+            // the CTAs' moments in rank order
+            double n = 0.0, mean = 0.0, m2 = 0.0;
+            for (int q = 0; q < q_n; ++q) {
+                const int64_t left = a.spatial - q * a.rows;
+                if (left <= 0) break;
+                const double k = (double)(left < a.rows ? left : a.rows) * (double)cg, t = n + k;
+                const double2 s = gn_peer_f64x2(gs + g, (unsigned)q);
+                const double d = s.x - mean;
+                mean += d * (k / t);
+                m2 += s.y + d * d * (n * k / t);
+                n = t;
+            }
+            gm[g] = (float)mean;
+            gr[g] = (float)rsqrt(m2 / n + (double)a.eps);
+        }
+        gn_cluster_arrive();  // met again at the end: no CTA leaves while its moments may be read
+    }
+    __syncthreads();
+    if (p.r0 == 0)  // the unit's first CTA
+        for (int g = threadIdx.x; g < p.ng; g += nt) {
+            a.mean[p.b * a.groups + p.g0 + g] = gm[g];
+            a.rstd[p.b * a.groups + p.g0 + g] = gr[g];
+        }
 
     T *y = static_cast<T *>(a.y) + (p.b * a.spatial + p.r0) * a.filters + p.c0;
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
-        float m[N], rs[N], sc[N], bi[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int g = (col * N + j) / cg;
-            m[j] = gm[g];
-            rs[j] = gr[g];
-            sc[j] = a.scales[p.c0 + col * N + j];
-            bi[j] = a.biases[p.c0 + col * N + j];
-        }
+        Affine<N, UNI> k;
+        k.load(col, cg, gm, gr, a.scales + p.c0, a.biases + p.c0);
+        const T *src = slab + rl * p.cb + col * N;
+        T *dst = y + (int64_t)rl * a.filters + (int64_t)col * N;
 #pragma unroll 2
         for (int r = rl; r < p.nr; r += rl_n) {
-            float f[N];
-            V::unpack(*reinterpret_cast<const Raw *>(slab + r * p.cb + col * N), f);
+            float2 f[P];
+            V::unpack(*reinterpret_cast<const Raw *>(src), f);
 #pragma unroll
-            for (int j = 0; j < N; ++j) f[j] = act_fwd<A>(__fmaf_rn((f[j] - m[j]) * rs[j], sc[j], bi[j]), a.act);
-            *reinterpret_cast<Raw *>(y + (int64_t)r * a.filters + (int64_t)col * N) = V::pack(f);
+            for (int i = 0; i < P; ++i) {
+                f[i] = k.z(f[i], i);
+                f[i] = make_float2(act_quick<A>(f[i].x, a.act), act_quick<A>(f[i].y, a.act));
+            }
+            *reinterpret_cast<Raw *>(dst) = V::pack(f);
+            src += rl_n * p.cb;
+            dst += pitch;
         }
     }
+    if (q_n > 1) gn_cluster_wait();
 }
 
 // Streaming path: merges the row chunks' (mean, M2) of a group (Chan, Golub and LeVeque's pairwise
@@ -203,7 +249,8 @@ __global__ void __launch_bounds__(256) k_gn_merge(const __grid_constant__ GnFwd 
     for (int64_t q = lane; q < a.chunks; q += 32) {
         const int64_t left = a.spatial - q * a.rows;
         const double k = (double)(left < a.rows ? left : a.rows) * (double)a.cg;
-        t.add(k, a.pieces[(i * a.chunks + q) * 2], a.pieces[(i * a.chunks + q) * 2 + 1]);
+        const double2 piece = a.pieces[i * a.chunks + q];
+        t.add(k, piece.x, piece.y);
     }
     for (int o = 16; o > 0; o >>= 1) {
         const double n = __shfl_down_sync(0xffffffffu, t.n, o), m = __shfl_down_sync(0xffffffffu, t.mean, o),
@@ -217,55 +264,45 @@ __global__ void __launch_bounds__(256) k_gn_merge(const __grid_constant__ GnFwd 
 }
 
 // Streaming path: the outputs, with the statistics from global memory.
-template <class T, int VB, int A>
+template <class T, int VB, int A, bool UNI>
 __global__ void __launch_bounds__(256) k_gn_apply(const __grid_constant__ GnFwd a) {
-    using V = Vec<T, VB>;
+    using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
-    constexpr int N = V::N;
+    constexpr int N = V::N, P = V::P;
     const Place p = place_of(a, a.chunks);
     const int nt = blockDim.x, v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
     if (rl >= rl_n) return;
-    const int cg = (int)a.cg;
-    const int64_t base = (p.b * a.spatial + p.r0) * a.filters + p.c0;
-    const T *x = static_cast<const T *>(a.x) + base;
-    T *y = static_cast<T *>(a.y) + base;
+    const int64_t base = (p.b * a.spatial + p.r0) * a.filters + p.c0, g0 = p.b * a.groups + p.g0;
     for (int col = col0; col < v; col += vp) {
-        float m[N], rs[N], sc[N], bi[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int64_t g = p.b * a.groups + p.g0 + (col * N + j) / cg;
-            m[j] = a.mean[g];
-            rs[j] = a.rstd[g];
-            sc[j] = a.scales[p.c0 + col * N + j];
-            bi[j] = a.biases[p.c0 + col * N + j];
-        }
+        Affine<N, UNI> k;
+        k.load(col, (int)a.cg, a.mean + g0, a.rstd + g0, a.scales + p.c0, a.biases + p.c0);
 #pragma unroll 4
         for (int r = rl; r < p.nr; r += rl_n) {
-            const int64_t at = (int64_t)r * a.filters + (int64_t)col * N;
-            float f[N];
-            V::unpack(*reinterpret_cast<const Raw *>(x + at), f);
+            const int64_t at = base + (int64_t)r * a.filters + (int64_t)col * N;
+            float2 f[P];
+            V::unpack(*reinterpret_cast<const Raw *>(static_cast<const T *>(a.x) + at), f);
 #pragma unroll
-            for (int j = 0; j < N; ++j) f[j] = act_fwd<A>(__fmaf_rn((f[j] - m[j]) * rs[j], sc[j], bi[j]), a.act);
-            *reinterpret_cast<Raw *>(y + at) = V::pack(f);
+            for (int i = 0; i < P; ++i) {
+                f[i] = k.z(f[i], i);
+                f[i] = make_float2(act_quick<A>(f[i].x, a.act), act_quick<A>(f[i].y, a.act));
+            }
+            *reinterpret_cast<Raw *>(static_cast<T *>(a.y) + at) = V::pack(f);
         }
     }
 }
 
-template <class T, int VB, int A>
+template <class T, int VB, int A, bool UNI>
 dnb_status run_fwd(GnFwd a, const GnPlan &p, int64_t batch, const DeviceState *ds, cudaStream_t s) {
     const char *what = "gn_act_forward";
     const int64_t units = batch * p.nu;
-    if (!p.stream) {
-        static std::atomic<int> opted[kMaxDevices];
-        return gn_launch(k_gn_fwd<T, VB, A, false>, a, units * p.cluster, p, ds, s, opted, what);
-    }
-    static std::atomic<int> opted[kMaxDevices];
-    DNB_TRY(gn_launch(k_gn_fwd<T, VB, A, true>, a, units * p.chunks, p, ds, s, opted, what));
+    static std::atomic<int> opted[2][kMaxDevices];
+    if (!p.stream) return gn_launch(k_gn_fwd<T, VB, A, UNI, false>, a, units * p.cluster, p, ds, s, opted[0], what);
+    DNB_TRY(gn_launch(k_gn_fwd<T, VB, -1, UNI, true>, a, units * p.chunks, p, ds, s, opted[1], what));
     const int64_t total = batch * a.groups;
     k_gn_merge<<<(unsigned)((total + 7) / 8), 256, 0, s>>>(a, total);
     DNB_TRY(after_launch(s, what));
-    k_gn_apply<T, VB, A><<<(unsigned)(units * p.chunks), p.threads, 0, s>>>(a);
+    k_gn_apply<T, VB, A, UNI><<<(unsigned)(units * p.chunks), p.threads, 0, s>>>(a);
     return after_launch(s, what);
 }
 
@@ -288,7 +325,7 @@ dnb_status dnb_gn_act_forward_workspace(const void *x, const void *y, int dtype,
     *bytes = 0;
     if (batch == 0 || spatial == 0) return DNB_OK;
     const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y);
-    const GnPlan p = gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, 1, 1);
+    const GnPlan p = gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, 1, false);
     if (p.stream) *bytes = (size_t)(batch * groups * p.chunks) * 16;
     return DNB_OK;
 }
@@ -308,7 +345,7 @@ dnb_status dnb_gn_act_forward(const void *x, void *y, int dtype, int64_t batch, 
     if ((x != y && overlaps(x, bytes, y, bytes)) || overlaps(mean, st, rstd, st) || overlaps(mean, st, y, bytes) ||
         overlaps(rstd, st, y, bytes) || overlaps(mean, st, x, bytes) || overlaps(rstd, st, x, bytes))
         return fail(DNB_ERR_INVALID, "%s: overlapping tensors", what);
-    const GnPlan p = gn_plan(batch, spatial, filters, groups, e, align, 1, 1);
+    const GnPlan p = gn_plan(batch, spatial, filters, groups, e, align, 1, false);
     const size_t need = p.stream ? (size_t)(batch * groups * p.chunks) * 16 : 0;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(DNB_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what, need,
@@ -323,7 +360,7 @@ dnb_status dnb_gn_act_forward(const void *x, void *y, int dtype, int64_t batch, 
     a.biases = biases;
     a.mean = mean;
     a.rstd = rstd;
-    a.pieces = static_cast<double *>(workspace);
+    a.pieces = static_cast<double2 *>(workspace);
     a.spatial = spatial;
     a.filters = filters;
     a.groups = groups;
@@ -336,12 +373,15 @@ dnb_status dnb_gn_act_forward(const void *x, void *y, int dtype, int64_t batch, 
     a.act = act;
     a.cluster = p.cluster;
     a.slab = (unsigned)p.slab;
-    a.part = (unsigned)p.part_floats;
+    a.part = (unsigned)p.part;
     return dispatch_dtype(dtype, [&]<class T>() -> dnb_status {
+        if (p.vb == 16 && p.uni)
+            return dispatch_act(act, [&]<int A>() { return run_fwd<T, 16, A, true>(a, p, batch, ds, s); });
         if (p.vb == 16)
-            return dispatch_act(act, [&]<int A>() { return run_fwd<T, 16, A>(a, p, batch, ds, s); });
-        if (p.vb == 4) return run_fwd<T, 4, -1>(a, p, batch, ds, s);
-        return run_fwd<T, (int)sizeof(T), -1>(a, p, batch, ds, s);
+            return dispatch_act(act, [&]<int A>() { return run_fwd<T, 16, A, false>(a, p, batch, ds, s); });
+        if (p.vb == 4)
+            return dispatch_act(act, [&]<int A>() { return run_fwd<T, 4, A, sizeof(T) == 4>(a, p, batch, ds, s); });
+        return run_fwd<T, (int)sizeof(T), -1, true>(a, p, batch, ds, s);
     });
 }
 

@@ -9,7 +9,8 @@
 //
 // A thread owns one vector of channels (VB bytes) and every RL-th row, so per-channel values sit in its
 // registers: V = cb / N vectors make a row; RL = T / V threads share a column, or, where a row is longer
-// than the block, the block walks the columns in passes of T vectors.
+// than the block, the block walks the columns in passes of T vectors. Where a group is a whole number of
+// vectors (`uni`), what belongs to the group is one value per thread instead of one per channel.
 #pragma once
 
 #include <atomic>
@@ -26,15 +27,16 @@ struct GnPlan {
     int64_t rows = 0;       // rows of a CTA
     int threads = 256;
     bool stream = false;
+    bool uni = false;       // a vector's channels are of one group
     int64_t chunks = 1;     // row chunks of a unit on the streaming path
     size_t slab = 0;        // bytes of one tensor's rows in shared memory, rounded to 16
-    size_t part_floats = 0; // floats of one per-thread partial array
+    size_t part = 0;        // entries of a per-thread partial array
     size_t smem = 0;
 };
 
 constexpr size_t kGnSmemTarget = 100 * 1024;  // two CTAs an SM
 constexpr size_t kGnSmemMax = 200 * 1024;
-constexpr size_t kGnStreamSlab = 32 * 1024;   // a streaming chunk's rows
+constexpr size_t kGnStreamBytes = 64 * 1024;  // a streaming chunk's inputs
 constexpr int kGnMaxCluster = 8;
 constexpr int64_t kGnMaxGroup = 4096;         // channels of a group: a row of them, with the partials, fits an SM
 
@@ -59,10 +61,9 @@ inline int64_t gcd64(int64_t a, int64_t b) {
     return a;
 }
 
-// tensors: inputs held in shared memory (1 forward, 2 or 3 backward); parts: per-thread partial arrays
-// (1 forward, 2 backward); align: the OR of the tensors' addresses.
+// tensors: inputs held in shared memory (1 forward, 2 or 3 backward); align: the OR of the tensors' addresses.
 inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t groups, int64_t esize, uintptr_t align,
-                      int tensors, int parts) {
+                      int tensors, bool backward) {
     constexpr int sms = 148;  // a B200's; the plan must not depend on the current device, for the workspace's size
     GnPlan p;
     const int64_t cg = filters / groups;
@@ -72,26 +73,33 @@ inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t g
     if (p.vb / esize / gcd64(p.vb / esize, cg) * cg > kGnMaxGroup) p.vb = (int)esize;
     const int64_t n = p.vb / esize;
     const int64_t step = n / gcd64(n, cg);
+    p.uni = cg % n == 0 && (p.vb == 16 || n == 1);  // the narrower vectors' kernels take channels one by one
     auto cap = [&](int64_t g) { return g < groups ? g : groups; };
     int64_t per = cap(step * ((64 + step * cg * esize - 1) / (step * cg * esize)));
     auto slab_of = [&](int64_t g, int64_t rows) { return (size_t)((rows * g * cg * esize + 15) / 16 * 16); };
     auto units_of = [&](int64_t g) { return batch * ((groups + g - 1) / g); };
     // short planes: wider units, while they still fill the SMs twice
-    while (per < groups && cap(2 * per) * cg <= 2048 && slab_of(cap(2 * per), spatial) * tensors <= 16 * 1024 && units_of(cap(2 * per)) >= 2 * sms)
+    while (per < groups && cap(2 * per) * cg <= 2048 && slab_of(cap(2 * per), spatial) * tensors <= 16 * 1024 &&
+           units_of(cap(2 * per)) >= 2 * sms)
         per = cap(2 * per);
     // rows narrower than 64 bytes rather than a second read of the inputs
     if (slab_of(per, (spatial + kGnMaxCluster - 1) / kGnMaxCluster) * tensors > kGnSmemMax && step < per) per = cap(step);
     p.cb = per * cg;
     p.nu = (groups + per - 1) / per;
+    auto sizes = [&](size_t slabs) {
+        const int64_t v = p.cb / n, wide = p.threads > v ? p.threads : v;
+        // forward: two floats a thread and vector (or channel), two doubles and two floats a group;
+        // backward: two floats a channel of a thread, two a thread (slices), two a channel, two a group
+        p.part = (size_t)(backward || !p.uni ? wide * n : wide);
+        p.smem = p.slab * slabs + p.part * 8 + 64;
+        p.smem += backward ? (size_t)p.threads * 8 + (size_t)p.cb * 8 + (size_t)per * 8 : (size_t)per * 24;
+    };
     auto shape = [&](int q) {
         p.cluster = q;
         p.rows = (spatial + q - 1) / q;
         p.slab = slab_of(per, p.rows);
         p.threads = p.slab * tensors > 64 * 1024 ? 512 : 256;
-        const int64_t v = p.cb / n;
-        p.part_floats = (size_t)(v >= p.threads ? p.cb : p.threads * n);  // of a narrower last unit too
-        // partial arrays; then per channel two floats, per group four doubles
-        p.smem = p.slab * tensors + p.part_floats * 4 * parts + (size_t)p.cb * 8 + (size_t)per * 32 + 64;
+        sizes((size_t)tensors);
     };
     int q = 1;
     shape(q);
@@ -99,18 +107,12 @@ inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t g
     if (p.smem > kGnSmemMax) {
         p.stream = true;
         p.cluster = 1;
-        int64_t rows = (int64_t)(kGnStreamSlab / (size_t)(p.cb * esize * tensors));
-        if (rows < 1) rows = 1;
-        p.rows = rows;
-        p.chunks = (spatial + rows - 1) / rows;
-        const int64_t chunks = p.chunks;
-        // shared memory of a chunk: the partials alone where one row is all that fits
-        p.slab = slab_of(per, rows);
+        p.rows = (int64_t)(kGnStreamBytes / (size_t)(p.cb * esize * tensors));
+        if (p.rows < 1) p.rows = 1;
+        p.chunks = (spatial + p.rows - 1) / p.rows;
+        p.slab = 0;
         p.threads = 256;
-        const int64_t v = p.cb / n;
-        p.part_floats = (size_t)(v >= p.threads ? p.cb : p.threads * n);
-        p.smem = p.slab * tensors + p.part_floats * 4 * parts + (size_t)p.cb * 8 + (size_t)per * 32 + 64;
-        p.chunks = chunks;
+        sizes(0);
         return p;
     }
     // few units: more CTAs for each, while a CTA keeps 8 KB
@@ -140,30 +142,66 @@ __device__ __forceinline__ Place place_of(const Args &a, int64_t per_unit) {
     return p;
 }
 
-__device__ __forceinline__ unsigned gn_cluster_rank() {
-    unsigned r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
+__device__ __forceinline__ void gn_cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void gn_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void gn_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The address of `p` (shared memory) in the cluster's CTA `rank`.
 __device__ __forceinline__ uint32_t gn_peer(const void *p, unsigned rank) {
     uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
     return r;
 }
-__device__ __forceinline__ double gn_peer_f64(const void *p, unsigned rank) {
-    double v;
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(gn_peer(p, rank)) : "memory");
+__device__ __forceinline__ double2 gn_peer_f64x2(const void *p, unsigned rank) {
+    double2 v;
+    asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "r"(gn_peer(p, rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ float gn_peer_f32(const void *p, unsigned rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(gn_peer(p, rank)) : "memory");
+__device__ __forceinline__ float2 gn_peer_f32x2(const void *p, unsigned rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(gn_peer(p, rank)) : "memory");
     return v;
 }
+// The local group of each channel of the vector at column `col`, in order (one division a vector).
+template <int N>
+__device__ __forceinline__ void groups_of(int col, int cg, int (&g)[N]) {
+    g[0] = col * N / cg;
+    int left = cg - (col * N - g[0] * cg);
+#pragma unroll
+    for (int j = 1; j < N; ++j) {
+        const bool next = --left == 0;
+        g[j] = g[j - 1] + next;
+        if (next) left = cg;
+    }
+}
+
+// z = (x - mean)*(rstd*scale) + bias for a vector's channels; the forward and the backward's recomputed output
+// share it, so that both see the same z.
+template <int N, bool UNI>
+struct Affine {
+    static constexpr int P = (N + 1) / 2;
+    float2 m[UNI ? 1 : P], k[P], b[P];
+    __device__ __forceinline__ void load(int col, int cg, const float *mean, const float *rstd, const float *scales,
+                                         const float *biases) {
+        int g[N];
+        if constexpr (!UNI) groups_of<N>(col, cg, g);
+        const int lg = UNI ? col * N / cg : 0;
+        const float um = UNI ? mean[lg] : 0.0f, ur = UNI ? rstd[lg] : 0.0f;
+        if constexpr (UNI) m[0] = both(-um);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int c = col * N + 2 * i;
+            const bool two = 2 * i + 1 < N;
+            if constexpr (!UNI) m[i] = make_float2(-mean[g[2 * i]], two ? -mean[g[two ? 2 * i + 1 : 0]] : 0.0f);
+            k[i] = make_float2((UNI ? ur : rstd[g[2 * i]]) * scales[c],
+                               two ? (UNI ? ur : rstd[g[two ? 2 * i + 1 : 0]]) * scales[c + 1] : 0.0f);
+            b[i] = make_float2(biases[c], two ? biases[c + 1] : 0.0f);
+        }
+    }
+    __device__ __forceinline__ float2 z(float2 x, int i) const {
+        return __ffma2_rn(__fadd2_rn(x, m[UNI ? 0 : i]), k[i], b[i]);
+    }
+};
 
 // Launches a GN kernel with its shared memory and cluster size.
 template <class K, class Args>

@@ -6,9 +6,10 @@
 // Both group sums are sums over the group's channels of scale * (the channel's sums over the rows), and
 // those channel sums, added over the images, are the updates: one reduction serves all four. Bound by
 // memory: x, delta (and y) in, dx out. k_gn_bwd keeps a unit (see dnb_gn.cuh) of each input in shared
-// memory: the channel sums are formed while it is loaded, dx from shared memory. A channel's rows are
-// added in fp32 per thread (rows / RL terms), across threads, CTAs and images in fp64, in a fixed order;
-// k_gn_updates adds the images up.
+// memory: the channel sums are formed while it is loaded, dx = d*k - (x - mean)*c2 - c1 from shared memory
+// (k = rstd*scale, c1 = rstd*sum(t)/n, c2 = rstd^2*sum(t*xh)/n: two fused multiply-adds an element).
+// A channel's rows are added in fp32 per thread (rows / RL terms), across threads, CTAs and images in fp64,
+// in a fixed order; k_gn_updates adds the images up.
 #include "dnb_gn.cuh"
 
 namespace dnb {
@@ -26,158 +27,206 @@ struct GnBwd {
     unsigned slab, part;
 };
 
-// The activation's gradient times delta, from the given output or the recomputed one.
+// The activation's gradient times delta, from the given output or the recomputed one (z: its argument).
 template <int A, bool Y>
-__device__ __forceinline__ float through(float delta, float y, float xh, float sc, float bi, int act) {
-    const float out = Y ? y : act_fwd<A>(__fmaf_rn(xh, sc, bi), act);
-    return delta * act_grad<A>(out, act);
+__device__ __forceinline__ float through(float delta, float y, float z, int act) {
+    if constexpr (A == DNB_ACT_LINEAR) return delta;
+    return delta * act_grad<A>(Y ? y : act_quick<A>(z, act), act);
 }
 
-template <class T, int VB, int A, bool Y, bool STREAM>
+// The group's (c1, c2) for a vector's channels.
+template <int N, bool UNI>
+__device__ __forceinline__ void load_moments(int col, int cg, const float2 *mo, float2 *c1, float2 *c2) {
+    if constexpr (UNI) {
+        const float2 m = mo[col * N / cg];
+        c1[0] = both(m.x);
+        c2[0] = both(m.y);
+    } else {
+        int g[N];
+        groups_of<N>(col, cg, g);
+#pragma unroll
+        for (int i = 0; i < (N + 1) / 2; ++i) {
+            const float2 m = mo[g[2 * i]], n = 2 * i + 1 < N ? mo[g[2 * i + 1 < N ? 2 * i + 1 : 0]] : both(0.0f);
+            c1[i] = make_float2(m.x, n.x);
+            c2[i] = make_float2(m.y, n.y);
+        }
+    }
+}
+// dx of a vector, in place of x.
+template <int P, int A, bool Y, bool UNI, class K>
+__device__ __forceinline__ void dx_of(float2 (&fx)[P], const float2 (&fd)[P], const float2 (&fy)[P], const K &k,
+                                      const float2 *c1, const float2 *c2, int act) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const float2 z = Y ? fy[i] : k.z(fx[i], i);
+        const float2 d = make_float2(through<A, Y>(fd[i].x, fy[i].x, z.x, act), through<A, Y>(fd[i].y, fy[i].y, z.y, act));
+        const float2 xm = __fadd2_rn(fx[i], k.m[UNI ? 0 : i]);
+        fx[i] = __ffma2_rn(d, k.k[i], __ffma2_rn(xm, c2[UNI ? 0 : i], c1[UNI ? 0 : i]));
+    }
+}
+
+template <class T, int VB, int A, bool Y, bool UNI, bool STREAM>
 __global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a) {
-    using V = Vec<T, VB>;
+    using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
-    constexpr int N = V::N;
+    constexpr int N = V::N, P = V::P;
     extern __shared__ __align__(16) unsigned char smem[];
     const Place p = place_of(a, STREAM ? a.chunks : a.cluster);
     T *sx = reinterpret_cast<T *>(smem), *sd = reinterpret_cast<T *>(smem + a.slab),
       *sy = reinterpret_cast<T *>(smem + 2 * a.slab);
     float *part = reinterpret_cast<float *>(smem + (STREAM ? 0u : (Y ? 3u : 2u) * a.slab));
-    float2 *ch = reinterpret_cast<float2 *>(part + ((2 * a.part + 3) & ~3u));  // the CTA's channel sums
-    float *m0 = reinterpret_cast<float *>(ch + p.cb), *m1 = m0 + p.ng;
-    const int nt = blockDim.x, v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
+    float2 *slices = reinterpret_cast<float2 *>(part + 2 * a.part);
+    const int nt = blockDim.x;
+    float2 *ch = slices + nt;                                    // the channels' sums
+    float2 *mo = ch + p.cb;                                      // the groups' (c1, c2)
+    const int v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
     const bool on = rl < rl_n;
-    const int64_t base = (p.b * a.spatial + p.r0) * a.filters + p.c0;
-    const T *x = static_cast<const T *>(a.x) + base, *delta = static_cast<const T *>(a.delta) + base;
-    const T *y = Y ? static_cast<const T *>(a.y) + base : nullptr;
-    const int cg = (int)a.cg;
+    const int64_t base = (p.b * a.spatial + p.r0) * a.filters + p.c0, g0 = p.b * a.groups + p.g0;
+    const int64_t pitch = a.filters * rl_n;
+    const int cg = (int)a.cg, srow = rl_n * p.cb;
 
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
-        float s0[N] = {}, s1[N] = {}, m[N], rs[N], sc[N], bi[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int64_t g = p.b * a.groups + p.g0 + (col * N + j) / cg;
-            m[j] = a.mean[g];
-            rs[j] = a.rstd[g];
-            sc[j] = Y ? 0.0f : a.scales[p.c0 + col * N + j];
-            bi[j] = Y ? 0.0f : a.biases[p.c0 + col * N + j];
-        }
-#pragma unroll 4
+        Affine<N, UNI> k;
+        k.load(col, cg, a.mean + g0, a.rstd + g0, a.scales + p.c0, a.biases + p.c0);
+        float2 s0[P] = {}, s1[P] = {};
+        const int64_t at = base + (int64_t)rl * a.filters + (int64_t)col * N;
+        const T *x = static_cast<const T *>(a.x) + at, *delta = static_cast<const T *>(a.delta) + at;
+        const T *y = Y ? static_cast<const T *>(a.y) + at : nullptr;
+        int in = rl * p.cb + col * N;
+#pragma unroll 2
         for (int r = rl; r < p.nr; r += rl_n) {
-            const int64_t at = (int64_t)r * a.filters + (int64_t)col * N;
-            const int in = r * p.cb + col * N;
-            const Raw rx = *reinterpret_cast<const Raw *>(x + at), rd = *reinterpret_cast<const Raw *>(delta + at);
+            const Raw rx = *reinterpret_cast<const Raw *>(x), rd = *reinterpret_cast<const Raw *>(delta);
             Raw ry{};
-            if constexpr (Y) ry = *reinterpret_cast<const Raw *>(y + at);
-            float fx[N], fd[N], fy[N] = {};
-            V::unpack(rx, fx);
-            V::unpack(rd, fd);
-            if constexpr (Y) V::unpack(ry, fy);
+            if constexpr (Y) {
+                ry = *reinterpret_cast<const Raw *>(y);
+                y += pitch;
+            }
+            x += pitch;
+            delta += pitch;
             if constexpr (!STREAM) {
                 *reinterpret_cast<Raw *>(sx + in) = rx;
                 *reinterpret_cast<Raw *>(sd + in) = rd;
                 if constexpr (Y) *reinterpret_cast<Raw *>(sy + in) = ry;
+                in += srow;
             }
+            float2 fx[P], fd[P], fy[P] = {};
+            V::unpack(rx, fx);
+            V::unpack(rd, fd);
+            if constexpr (Y) V::unpack(ry, fy);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float xh = (fx[j] - m[j]) * rs[j];
-                const float d = through<A, Y>(fd[j], fy[j], xh, sc[j], bi[j], a.act);
-                s0[j] += d;
-                s1[j] = __fmaf_rn(d, xh, s1[j]);
+            for (int i = 0; i < P; ++i) {
+                const float2 z = Y ? fy[i] : k.z(fx[i], i);
+                const float2 d = make_float2(through<A, Y>(fd[i].x, fy[i].x, z.x, a.act),
+                                             through<A, Y>(fd[i].y, fy[i].y, z.y, a.act));
+                s0[i] = __fadd2_rn(s0[i], d);
+                s1[i] = __ffma2_rn(d, __fadd2_rn(fx[i], k.m[UNI ? 0 : i]), s1[i]);
             }
         }
+        int g[N];
+        groups_of<N>(col, cg, g);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            part[rl * p.cb + col * N + j] = s0[j];
-            part[a.part + rl * p.cb + col * N + j] = s1[j];
+            part[rl * p.cb + col * N + j] = j & 1 ? s0[j / 2].y : s0[j / 2].x;
+            part[a.part + rl * p.cb + col * N + j] = (j & 1 ? s1[j / 2].y : s1[j / 2].x) * a.rstd[g0 + g[j]];
         }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < p.cb; c += nt) {
+    // a channel's sums: its row lanes in slices, one thread each, then the slices
+    const int sl_n = p.cb < nt ? min(nt / p.cb, rl_n) : 1;
+    for (int t = threadIdx.x; t < p.cb * sl_n; t += nt) {
+        const int c = t % p.cb, sl = t / p.cb;
         double s0 = 0.0, s1 = 0.0;
-        for (int r = 0; r < rl_n; ++r) {
+        for (int r = sl; r < rl_n; r += sl_n) {
             s0 += (double)part[r * p.cb + c];
             s1 += (double)part[a.part + r * p.cb + c];
         }
         const float2 s = make_float2((float)s0, (float)s1);
-        if constexpr (STREAM)
-            a.pieces[(p.b * a.chunks + blockIdx.x % a.chunks) * a.filters + p.c0 + c] = s;
-        else
-            ch[c] = s;
+        if (sl_n == 1) ch[c] = s;
+        else slices[sl * p.cb + c] = s;
     }
-    if constexpr (STREAM) return;
+    __syncthreads();
+    if (sl_n > 1) {
+        for (int c = threadIdx.x; c < p.cb; c += nt) {
+            double s0 = 0.0, s1 = 0.0;
+            for (int sl = 0; sl < sl_n; ++sl) {
+                const float2 s = slices[sl * p.cb + c];
+                s0 += (double)s.x;
+                s1 += (double)s.y;
+            }
+            ch[c] = make_float2((float)s0, (float)s1);
+        }
+        if (STREAM || a.cluster == 1) __syncthreads();
+    }
+    if constexpr (STREAM) {
+        for (int c = threadIdx.x; c < p.cb; c += nt)
+            a.pieces[(p.b * a.chunks + blockIdx.x % a.chunks) * a.filters + p.c0 + c] = ch[c];
+        return;
+    }
     const int q_n = a.cluster;
+    float2 *all = ch;
     if (q_n > 1) {  // the unit's sums: every CTA adds the CTAs' in rank order, into its (now free) partials
-        gn_cluster_sync();
+        gn_cluster_arrive();
+        gn_cluster_wait();
+        all = reinterpret_cast<float2 *>(part);
         for (int c = threadIdx.x; c < p.cb; c += nt) {
             double s0 = 0.0, s1 = 0.0;
             for (int q = 0; q < q_n; ++q) {
-                s0 += (double)gn_peer_f32(&ch[c].x, (unsigned)q);
-                s1 += (double)gn_peer_f32(&ch[c].y, (unsigned)q);
+                const float2 s = gn_peer_f32x2(ch + c, (unsigned)q);
+                s0 += (double)s.x;
+                s1 += (double)s.y;
             }
-            part[c] = (float)s0;
-            part[a.part + c] = (float)s1;
+            all[c] = make_float2((float)s0, (float)s1);
         }
-        gn_cluster_sync();  // no CTA overwrites or leaves before its peers have read it
-        for (int c = threadIdx.x; c < p.cb; c += nt) ch[c] = make_float2(part[c], part[a.part + c]);
+        gn_cluster_arrive();  // met again at the end: no CTA leaves while its sums may be read
+        __syncthreads();
     }
-    __syncthreads();
     if (p.r0 == 0)
-        for (int c = threadIdx.x; c < p.cb; c += nt) a.image[p.b * a.filters + p.c0 + c] = ch[c];
+        for (int c = threadIdx.x; c < p.cb; c += nt) a.image[p.b * a.filters + p.c0 + c] = all[c];
     const double count = (double)a.spatial * (double)a.cg;
     const int lane = threadIdx.x & 31;
     for (int g = threadIdx.x >> 5; g < p.ng; g += nt >> 5) {
         double s0 = 0.0, s1 = 0.0;
         for (int c = lane; c < cg; c += 32) {
             const double sc = (double)a.scales[p.c0 + g * cg + c];
-            s0 += sc * (double)ch[g * cg + c].x;
-            s1 += sc * (double)ch[g * cg + c].y;
+            s0 += sc * (double)all[g * cg + c].x;
+            s1 += sc * (double)all[g * cg + c].y;
         }
         s0 = warp_sum(s0);
         s1 = warp_sum(s1);
         if (lane == 0) {
-            m0[g] = (float)(s0 / count);
-            m1[g] = (float)(s1 / count);
+            const double rs = (double)a.rstd[g0 + g];
+            mo[g] = make_float2((float)(-rs * s0 / count), (float)(-rs * rs * s1 / count));
         }
     }
     __syncthreads();
 
-    T *dx = static_cast<T *>(a.dx) + base;
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
-        float m[N], rs[N], sc[N], bi[N], k0[N], k1[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int lg = (col * N + j) / cg;
-            const int64_t g = p.b * a.groups + p.g0 + lg;
-            m[j] = a.mean[g];
-            rs[j] = a.rstd[g];
-            sc[j] = a.scales[p.c0 + col * N + j];
-            bi[j] = Y ? 0.0f : a.biases[p.c0 + col * N + j];
-            k0[j] = m0[lg];
-            k1[j] = m1[lg];
-        }
+        Affine<N, UNI> k;
+        k.load(col, cg, a.mean + g0, a.rstd + g0, a.scales + p.c0, a.biases + p.c0);
+        float2 c1[UNI ? 1 : P], c2[UNI ? 1 : P];
+        load_moments<N, UNI>(col, cg, mo, c1, c2);
+        T *dx = static_cast<T *>(a.dx) + base + (int64_t)rl * a.filters + (int64_t)col * N;
+        int in = rl * p.cb + col * N;
+#pragma unroll 2
         for (int r = rl; r < p.nr; r += rl_n) {
-            const int in = r * p.cb + col * N;
-            float fx[N], fd[N], fy[N] = {};
+            float2 fx[P], fd[P], fy[P] = {};
             V::unpack(*reinterpret_cast<const Raw *>(sx + in), fx);
             V::unpack(*reinterpret_cast<const Raw *>(sd + in), fd);
             if constexpr (Y) V::unpack(*reinterpret_cast<const Raw *>(sy + in), fy);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float xh = (fx[j] - m[j]) * rs[j];
-                const float d = through<A, Y>(fd[j], fy[j], xh, sc[j], bi[j], a.act);
-                fx[j] = rs[j] * (__fmaf_rn(d, sc[j], -k0[j]) - xh * k1[j]);
-            }
-            *reinterpret_cast<Raw *>(dx + (int64_t)r * a.filters + (int64_t)col * N) = V::pack(fx);
+            in += srow;
+            dx_of<P, A, Y, UNI>(fx, fd, fy, k, c1, c2, a.act);
+            *reinterpret_cast<Raw *>(dx) = V::pack(fx);
+            dx += pitch;
         }
     }
+    if (q_n > 1) gn_cluster_wait();
 }
 
 // Streaming path: a block per (image, group): the chunks' channel sums added in order, then the group's
-// two means.
+// (c1, c2).
 __global__ void __launch_bounds__(128) k_gn_bwd_merge(const __grid_constant__ GnBwd a) {
     __shared__ double red[2][4];
     const int64_t b = blockIdx.x / a.groups, g = blockIdx.x % a.groups;
@@ -205,64 +254,49 @@ __global__ void __launch_bounds__(128) k_gn_bwd_merge(const __grid_constant__ Gn
         const double n = (double)a.spatial * (double)a.cg;
         t0 = red[0][0] + red[0][1] + red[0][2] + red[0][3];
         t1 = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-        a.moments[blockIdx.x] = make_float2((float)(t0 / n), (float)(t1 / n));
+        const double rs = (double)a.rstd[blockIdx.x];
+        a.moments[blockIdx.x] = make_float2((float)(-rs * t0 / n), (float)(-rs * rs * t1 / n));
     }
 }
 
-template <class T, int VB, int A, bool Y>
+template <class T, int VB, int A, bool Y, bool UNI>
 __global__ void __launch_bounds__(256) k_gn_bwd_apply(const __grid_constant__ GnBwd a) {
-    using V = Vec<T, VB>;
+    using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
-    constexpr int N = V::N;
+    constexpr int N = V::N, P = V::P;
     const Place p = place_of(a, a.chunks);
     const int nt = blockDim.x, v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
     if (rl >= rl_n) return;
-    const int cg = (int)a.cg;
-    const int64_t base = (p.b * a.spatial + p.r0) * a.filters + p.c0;
-    const T *x = static_cast<const T *>(a.x) + base, *delta = static_cast<const T *>(a.delta) + base;
-    const T *y = Y ? static_cast<const T *>(a.y) + base : nullptr;
-    T *dx = static_cast<T *>(a.dx) + base;
+    const int64_t base = (p.b * a.spatial + p.r0) * a.filters + p.c0, g0 = p.b * a.groups + p.g0;
     for (int col = col0; col < v; col += vp) {
-        float m[N], rs[N], sc[N], bi[N], k0[N], k1[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int64_t g = p.b * a.groups + p.g0 + (col * N + j) / cg;
-            m[j] = a.mean[g];
-            rs[j] = a.rstd[g];
-            sc[j] = a.scales[p.c0 + col * N + j];
-            bi[j] = Y ? 0.0f : a.biases[p.c0 + col * N + j];
-            k0[j] = a.moments[g].x;
-            k1[j] = a.moments[g].y;
-        }
+        Affine<N, UNI> k;
+        k.load(col, (int)a.cg, a.mean + g0, a.rstd + g0, a.scales + p.c0, a.biases + p.c0);
+        float2 c1[UNI ? 1 : P], c2[UNI ? 1 : P];
+        load_moments<N, UNI>(col, (int)a.cg, a.moments + g0, c1, c2);
 #pragma unroll 2
         for (int r = rl; r < p.nr; r += rl_n) {
-            const int64_t at = (int64_t)r * a.filters + (int64_t)col * N;
-            float fx[N], fd[N], fy[N] = {};
-            V::unpack(*reinterpret_cast<const Raw *>(x + at), fx);
-            V::unpack(*reinterpret_cast<const Raw *>(delta + at), fd);
-            if constexpr (Y) V::unpack(*reinterpret_cast<const Raw *>(y + at), fy);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float xh = (fx[j] - m[j]) * rs[j];
-                const float d = through<A, Y>(fd[j], fy[j], xh, sc[j], bi[j], a.act);
-                fx[j] = rs[j] * (__fmaf_rn(d, sc[j], -k0[j]) - xh * k1[j]);
-            }
-            *reinterpret_cast<Raw *>(dx + at) = V::pack(fx);
+            const int64_t at = base + (int64_t)r * a.filters + (int64_t)col * N;
+            float2 fx[P], fd[P], fy[P] = {};
+            V::unpack(*reinterpret_cast<const Raw *>(static_cast<const T *>(a.x) + at), fx);
+            V::unpack(*reinterpret_cast<const Raw *>(static_cast<const T *>(a.delta) + at), fd);
+            if constexpr (Y) V::unpack(*reinterpret_cast<const Raw *>(static_cast<const T *>(a.y) + at), fy);
+            dx_of<P, A, Y, UNI>(fx, fd, fy, k, c1, c2, a.act);
+            *reinterpret_cast<Raw *>(static_cast<T *>(a.dx) + at) = V::pack(fx);
         }
     }
 }
 
-// The updates: a block per 32 channels, 8 slices of the images added in order, then the slices.
-__global__ void __launch_bounds__(256) k_gn_updates(const float2 *image, int64_t batch, int64_t filters,
-                                                    float *bias_updates, float *scale_updates, int add) {
-    __shared__ double red[2][8][32];
+// The updates: a block per 32 channels, 32 slices of the images (each added in order), then the slices.
+__global__ void __launch_bounds__(1024) k_gn_updates(const float2 *image, int64_t batch, int64_t filters,
+                                                     float *bias_updates, float *scale_updates, int add) {
+    __shared__ double red[2][32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + tx;
     double s0 = 0.0, s1 = 0.0;
     if (c < filters) {
 #pragma unroll 4
-        for (int64_t b = ty; b < batch; b += 8) {
+        for (int64_t b = ty; b < batch; b += 32) {
             const float2 v = image[b * filters + c];
             s0 += (double)v.x;
             s1 += (double)v.y;
@@ -271,13 +305,13 @@ __global__ void __launch_bounds__(256) k_gn_updates(const float2 *image, int64_t
     red[0][ty][tx] = s0;
     red[1][ty][tx] = s1;
     __syncthreads();
-    if (ty == 0 && c < filters) {
-        for (int k = 1; k < 8; ++k) {
-            s0 += red[0][k][tx];
-            s1 += red[1][k][tx];
-        }
-        bias_updates[c] = (float)(add ? (double)bias_updates[c] + s0 : s0);
-        scale_updates[c] = (float)(add ? (double)scale_updates[c] + s1 : s1);
+    // warp w: channel w's slices, a lane each
+    s0 = warp_sum(red[0][tx][ty]);
+    s1 = warp_sum(red[1][tx][ty]);
+    const int64_t o = (int64_t)blockIdx.x * 32 + ty;
+    if (tx == 0 && o < filters) {
+        bias_updates[o] = (float)(add ? (double)bias_updates[o] + s0 : s0);
+        scale_updates[o] = (float)(add ? (double)scale_updates[o] + s1 : s1);
     }
 }
 
@@ -298,23 +332,20 @@ GnPlan plan_bwd(const void *x, const void *y, const void *delta, const void *dx,
                 int64_t spatial, int64_t filters, int64_t groups) {
     const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) |
                             reinterpret_cast<uintptr_t>(delta) | reinterpret_cast<uintptr_t>(dx);
-    return gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, y ? 3 : 2, 2);
+    return gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, y ? 3 : 2, true);
 }
 
-template <class T, int VB, int A, bool Y>
+template <class T, int VB, int A, bool Y, bool UNI>
 dnb_status run_bwd(const GnBwd &a, const GnPlan &p, int64_t batch, const DeviceState *ds, cudaStream_t s) {
     const char *what = "gn_act_backward";
     const int64_t units = batch * p.nu;
-    if (!p.stream) {
-        static std::atomic<int> opted[kMaxDevices];
-        return gn_launch(k_gn_bwd<T, VB, A, Y, false>, a, units * p.cluster, p, ds, s, opted, what);
-    }
-    static std::atomic<int> opted[kMaxDevices];
-    DNB_TRY(gn_launch(k_gn_bwd<T, VB, A, Y, true>, a, units * p.chunks, p, ds, s, opted, what));
+    static std::atomic<int> opted[2][kMaxDevices];
+    if (!p.stream) return gn_launch(k_gn_bwd<T, VB, A, Y, UNI, false>, a, units * p.cluster, p, ds, s, opted[0], what);
+    DNB_TRY(gn_launch(k_gn_bwd<T, VB, A, Y, UNI, true>, a, units * p.chunks, p, ds, s, opted[1], what));
     if (batch * a.groups > 0x7fffffffll) return fail(DNB_ERR_UNSUPPORTED, "%s: too many groups", what);
     k_gn_bwd_merge<<<(unsigned)(batch * a.groups), 128, 0, s>>>(a);
     DNB_TRY(after_launch(s, what));
-    k_gn_bwd_apply<T, VB, A, Y><<<(unsigned)(units * p.chunks), p.threads, 0, s>>>(a);
+    k_gn_bwd_apply<T, VB, A, Y, UNI><<<(unsigned)(units * p.chunks), p.threads, 0, s>>>(a);
     return after_launch(s, what);
 }
 
@@ -358,7 +389,7 @@ dnb_status dnb_gn_act_backward(const void *x, const void *y, const void *delta, 
     if (batch == 0 || spatial == 0) {  // sums over nothing
         if (add) return DNB_OK;
         DNB_TRY(current_device(&ds));
-        k_gn_updates<<<ublocks, 256, 0, s>>>(nullptr, 0, filters, bias_updates, scale_updates, 0);
+        k_gn_updates<<<ublocks, 1024, 0, s>>>(nullptr, 0, filters, bias_updates, scale_updates, 0);
         return after_launch(s, what);
     }
     if (!x || !delta || !dx || !scales || !biases || !mean || !rstd)
@@ -401,18 +432,21 @@ dnb_status dnb_gn_act_backward(const void *x, const void *y, const void *delta, 
     a.act = act;
     a.cluster = p.cluster;
     a.slab = (unsigned)p.slab;
-    a.part = (unsigned)p.part_floats;
-    auto with_y = [&]<class T, int VB, int A>() {
-        return y ? run_bwd<T, VB, A, true>(a, p, batch, ds, s) : run_bwd<T, VB, A, false>(a, p, batch, ds, s);
+    a.part = (unsigned)p.part;
+    auto with_y = [&]<class T, int VB, int A, bool UNI>() {
+        return y ? run_bwd<T, VB, A, true, UNI>(a, p, batch, ds, s) : run_bwd<T, VB, A, false, UNI>(a, p, batch, ds, s);
     };
     const dnb_status st = dispatch_dtype(dtype, [&]<class T>() -> dnb_status {
+        if (p.vb == 16 && p.uni)
+            return dispatch_act(act, [&]<int A>() { return with_y.template operator()<T, 16, A, true>(); });
         if (p.vb == 16)
-            return dispatch_act(act, [&]<int A>() { return with_y.template operator()<T, 16, A>(); });
-        if (p.vb == 4) return with_y.template operator()<T, 4, -1>();
-        return with_y.template operator()<T, (int)sizeof(T), -1>();
+            return dispatch_act(act, [&]<int A>() { return with_y.template operator()<T, 16, A, false>(); });
+        if (p.vb == 4)
+            return dispatch_act(act, [&]<int A>() { return with_y.template operator()<T, 4, A, sizeof(T) == 4>(); });
+        return with_y.template operator()<T, (int)sizeof(T), -1, true>();
     });
     DNB_TRY(st);
-    k_gn_updates<<<ublocks, 256, 0, s>>>(a.image, batch, filters, bias_updates, scale_updates, add);
+    k_gn_updates<<<ublocks, 1024, 0, s>>>(a.image, batch, filters, bias_updates, scale_updates, add);
     return after_launch(s, what);
 }
 

@@ -85,6 +85,72 @@ struct Vec {
     }
 };
 
+// The same vector as pairs of floats, for the two-wide fp32 instructions (add, multiply and fused
+// multiply-add of a pair in one issue). A single element is a pair whose second half is 0.
+template <class T, int VB>
+struct Pairs {
+    static constexpr int N = VB / (int)sizeof(T), P = (N + 1) / 2;
+    using Raw = typename RawVec<VB>::type;
+    static __device__ __forceinline__ void unpack(const Raw &raw, float2 (&f)[P]) {
+        if constexpr (N == 1) {
+            float v[1];
+            Vec<T, VB>::unpack(raw, v);
+            f[0] = make_float2(v[0], 0.0f);
+        } else if constexpr (sizeof(T) == 4) {
+            float v[N];
+            Vec<T, VB>::unpack(raw, v);
+#pragma unroll
+            for (int i = 0; i < P; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+        } else {
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(&raw);
+#pragma unroll
+            for (int i = 0; i < P; ++i) f[i] = pair(w[i], static_cast<T *>(nullptr));
+        }
+    }
+    static __device__ __forceinline__ Raw pack(const float2 (&f)[P]) {
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i & 1 ? f[i / 2].y : f[i / 2].x;
+        if constexpr (N == 1 || sizeof(T) == 4) {
+            return Vec<T, VB>::pack(v);
+        } else {
+            Raw raw;
+            uint32_t *w = reinterpret_cast<uint32_t *>(&raw);
+#pragma unroll
+            for (int i = 0; i < P; ++i) w[i] = word(f[i], static_cast<T *>(nullptr));
+            return raw;
+        }
+    }
+    static __device__ __forceinline__ float2 pair(uint32_t w, __nv_bfloat16 *) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+    static __device__ __forceinline__ float2 pair(uint32_t w, __half *) {
+        return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    }
+    static __device__ __forceinline__ float2 pair(uint32_t, float *) { return make_float2(0.0f, 0.0f); }
+    static __device__ __forceinline__ uint32_t word(float2 f, __nv_bfloat16 *) {
+        const __nv_bfloat162 h = __float22bfloat162_rn(f);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ uint32_t word(float2 f, __half *) {
+        const __half2 h = __float22half2_rn(f);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ uint32_t word(float2, float *) { return 0u; }
+};
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
+
+// An activation of the 16-bit entries: the fp32 entries' (dnb_common.cuh), but for the logistic, whose
+// exponential and reciprocal are the special-function unit's (2 ulp each; a division and an exponential to
+// the last bit cost a third of a group norm's time and vanish in the rounding to 16 bits).
+template <int A>
+__device__ __forceinline__ float act_quick(float x, int a) {
+    if constexpr (A == DNB_ACT_LOGISTIC) return __fdividef(1.0f, 1.0f + __expf(-x));
+    else if constexpr (A == DNB_ACT_LEAKY) return fmaxf(x, 0.1f * x);
+    else return act_fwd<A>(x, a);
+}
+
 // Calls f.template operator()<T>() with the element type.
 template <class F>
 auto dispatch_dtype(int dtype, F &&f) {
