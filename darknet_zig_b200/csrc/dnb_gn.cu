@@ -7,9 +7,9 @@
 // into shared memory and adds it up on the way; y comes from shared memory. The sums are of d = x - s and
 // d^2 about a shift s of each thread's own, the first element it sees of the group: s is one of the group's
 // elements, so s's own distance from the mean is among the deviations that make up the variance, and no mean,
-// however far from 0, cancels. Each thread's (count, mean, squared deviations) are merged in fp64 (Chan,
-// Golub and LeVeque), in a fixed order. With a second walk over shared memory for the deviations instead,
-// [128,784,256] bf16 took 45 us, bound by instructions (30 an element against 9 now).
+// however far from 0, cancels. Each thread's (count, mean, squared deviations) are merged as Chan, Golub and LeVeque
+// do, about one of the means, in a fixed order. With a second walk over shared memory for the deviations instead,
+// [128,784,256] bf16 took 45 us, bound by instructions (30 an element).
 #include "dnb_gn.cuh"
 
 namespace dnb {
@@ -20,28 +20,43 @@ struct GnFwd {
     void *y;
     const float *scales, *biases;
     float *mean, *rstd;
-    double2 *pieces;  // streaming path: [batch][groups][chunks] = (mean, M2) of a row chunk
+    float2 *pieces;   // streaming path: [batch][groups][chunks] = (mean, M2) of a row chunk
     int64_t spatial, filters, groups, cg, cb, nu, rows, chunks;
-    float eps;
+    float eps, inv_count;  // 1 / n
     int act, cluster;
+    int unit_groups;
     unsigned slab, part;  // bytes, entries
+};
+
+// Moments (weight, mean, M2) added up about a reference mean `ref` that is one of theirs, in fp32: the
+// differences of the means are of the group's own spread, and small beside it.
+struct About {
+    float ref, n = 0.0f, s = 0.0f, q = 0.0f;
+    __device__ __forceinline__ void add(float w, float mean, float m2) {
+        const float d = mean - ref, wd = w * d;
+        n += w;
+        s += wd;
+        q += __fmaf_rn(wd, d, m2);
+    }
+    __device__ __forceinline__ float2 close() const {  // (mean, M2)
+        if (n == 0.0f) return make_float2(0.0f, 0.0f);
+        const float shift = s / n, m2 = __fmaf_rn(-shift, s, q);
+        return make_float2(ref + shift, m2 < 0.0f ? 0.0f : m2);
+    }
 };
 
 // Merges the moments of a group's threads: entries (rl, e) with e < eg of the group, each `per` elements of a
 // row times the thread's rows. A warp's lanes all get (mean, M2).
-__device__ __forceinline__ double2 merge_group(const float *mean, const float *m2, int rl_n, int pitch, int e0, int eg,
-                                               int per, int nr) {
-    const int lane = threadIdx.x & 31, total = rl_n * eg;
+__device__ __forceinline__ float2 merge_group(const float *mean, const float *m2, int rl_n, int pitch, int e0, int eg,
+                                              int per, int nr) {
+    const int lane = threadIdx.x & 31, total = rl_n * eg, full = nr / rl_n, rem = nr - full * rl_n;
     const int step_r = 32 / eg, step_e = 32 - step_r * eg;
-    double n = 0.0, s = 0.0;
+    About t;
+    t.ref = mean[e0];
     int r = lane / eg, e = lane - r * eg;
     for (int i = lane; i < total; i += 32) {
-        const int rows = nr > r ? (nr - r + rl_n - 1) / rl_n : 0;
-        const double w = (double)(rows * per);
-        if (rows) {
-            n += w;
-            s += w * (double)mean[r * pitch + e0 + e];
-        }
+        const int rows = full + (r < rem);
+        if (rows) t.add((float)(rows * per), mean[r * pitch + e0 + e], m2[r * pitch + e0 + e]);
         r += step_r;
         e += step_e;
         if (e >= eg) {
@@ -49,26 +64,10 @@ __device__ __forceinline__ double2 merge_group(const float *mean, const float *m
             ++r;
         }
     }
-    n = warp_sum(n);
-    s = warp_sum(s);
-    const double mu = n > 0.0 ? s / n : 0.0;
-    double q = 0.0;
-    r = lane / eg;
-    e = lane - r * eg;
-    for (int i = lane; i < total; i += 32) {
-        const int rows = nr > r ? (nr - r + rl_n - 1) / rl_n : 0;
-        if (rows) {
-            const double d = (double)mean[r * pitch + e0 + e] - mu;
-            q += (double)m2[r * pitch + e0 + e] + (double)(rows * per) * d * d;
-        }
-        r += step_r;
-        e += step_e;
-        if (e >= eg) {
-            e -= eg;
-            ++r;
-        }
-    }
-    return make_double2(mu, warp_sum(q));
+    t.n = warp_sum(t.n);
+    t.s = warp_sum(t.s);
+    t.q = warp_sum(t.q);
+    return t.close();
 }
 
 template <class T, int VB, int A, bool UNI, bool STREAM>
@@ -77,11 +76,12 @@ __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a)
     using Raw = typename V::Raw;
     constexpr int N = V::N, P = V::P;
     extern __shared__ __align__(16) unsigned char smem[];
-    const Place p = place_of(a, STREAM ? a.chunks : a.cluster);
+    const Place p = place_of(a, STREAM ? (unsigned)a.chunks : (unsigned)a.cluster);
     T *slab = reinterpret_cast<T *>(smem);
     float *pm = reinterpret_cast<float *>(smem + a.slab), *pq = pm + a.part;  // the threads' means and M2
-    double2 *gs = reinterpret_cast<double2 *>(smem + ((a.slab + a.part * 8 + 15) & ~15u));  // the CTA's, a group
+    float2 *gs = reinterpret_cast<float2 *>(smem + a.slab + a.part * 8);  // the CTA's, a group
     float *gm = reinterpret_cast<float *>(gs + p.ng), *gr = gm + p.ng;                       // mean, rstd
+    float *sc = gr + p.ng, *bi = sc + p.cb;
     const int nt = blockDim.x, v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
     const bool on = rl < rl_n;
@@ -89,12 +89,28 @@ __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a)
     const int cg = (int)a.cg;
     const int64_t pitch = a.filters * rl_n;
 
+    if constexpr (!STREAM) {
+        for (int col = col0; col < v; col += vp) {
+            if (!on) break;
+            const T *src = x + (int64_t)rl * a.filters + (int64_t)col * N;
+            T *dst = slab + rl * p.cb + col * N;
+#pragma unroll 4
+            for (int r = rl; r < p.nr; r += rl_n) {
+                gn_copy<VB>(dst, src);
+                src += pitch;
+                dst += rl_n * p.cb;
+            }
+        }
+        gn_stage_params(sc, a.scales, a.biases, p);
+        gn_arrived();
+    }
+
+    const int rows = p.nr > rl ? (p.nr - rl + rl_n - 1) / rl_n : 0;
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
         float2 s1[P] = {}, s2[P] = {}, sh[P] = {};
-        const T *src = x + (int64_t)rl * a.filters + (int64_t)col * N;
-        T *dst = slab + rl * p.cb + col * N;
-        const int rows = p.nr > rl ? (p.nr - rl + rl_n - 1) / rl_n : 0;
+        const T *src = STREAM ? x + (int64_t)rl * a.filters + (int64_t)col * N : slab + rl * p.cb + col * N;
+        const int64_t step = STREAM ? pitch : rl_n * p.cb;
         if (rows) {
             V::unpack(*reinterpret_cast<const Raw *>(src), sh);
             if constexpr (UNI) {
@@ -102,34 +118,11 @@ __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a)
                 for (int i = P - 1; i >= 0; --i) sh[i] = both(sh[0].x);
             }
         }
-        constexpr int U = 4;
-        int r = 0;
-        for (; r + U <= rows; r += U) {
-            Raw raw[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = *reinterpret_cast<const Raw *>(src + u * pitch);
-            src += U * pitch;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float2 f[P];
-                V::unpack(raw[u], f);
-                if constexpr (!STREAM) *reinterpret_cast<Raw *>(dst + u * rl_n * p.cb) = raw[u];
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const float2 d = __fadd2_rn(f[i], neg(sh[i]));
-                    s1[i] = __fadd2_rn(s1[i], d);
-                    s2[i] = __ffma2_rn(d, d, s2[i]);
-                }
-            }
-            dst += U * rl_n * p.cb;
-        }
-        for (; r < rows; ++r) {
-            const Raw raw = *reinterpret_cast<const Raw *>(src);
-            src += pitch;
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
             float2 f[P];
-            V::unpack(raw, f);
-            if constexpr (!STREAM) *reinterpret_cast<Raw *>(dst) = raw;
-            dst += rl_n * p.cb;
+            V::unpack(*reinterpret_cast<const Raw *>(src), f);
+            src += step;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const float2 d = __fadd2_rn(f[i], neg(sh[i]));
@@ -145,12 +138,12 @@ __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a)
                 s2[0] = __fadd2_rn(s2[0], s2[i]);
             }
             const float t1 = N > 1 ? s1[0].x + s1[0].y : s1[0].x, t2 = N > 1 ? s2[0].x + s2[0].y : s2[0].x;
-            const float inv = rows ? __fdividef(1.0f, (float)(rows * N)) : 0.0f;
+            const float inv = rows ? 1.0f / (float)(rows * N) : 0.0f;
             pm[rl * v + col] = __fmaf_rn(t1, inv, sh[0].x);
             const float q = __fmaf_rn(-t1 * inv, t1, t2);
             pq[rl * v + col] = q < 0.0f ? 0.0f : q;
         } else {
-            const float inv = rows ? __fdividef(1.0f, (float)rows) : 0.0f;
+            const float inv = rows ? 1.0f / (float)rows : 0.0f;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float t1 = j & 1 ? s1[j / 2].y : s1[j / 2].x, t2 = j & 1 ? s2[j / 2].y : s2[j / 2].x;
@@ -164,13 +157,13 @@ __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a)
     const int eg = UNI ? cg / N : cg, lane = threadIdx.x & 31;
     const int q_n = STREAM ? 1 : a.cluster;
     for (int g = threadIdx.x >> 5; g < p.ng; g += nt >> 5) {
-        const double2 s = merge_group(pm, pq, rl_n, UNI ? v : p.cb, g * eg, eg, UNI ? N : 1, p.nr);
+        const float2 s = merge_group(pm, pq, rl_n, UNI ? v : p.cb, g * eg, eg, UNI ? N : 1, p.nr);
         if (lane != 0) continue;
         if constexpr (STREAM) {
-            a.pieces[(p.b * a.groups + p.g0 + g) * a.chunks + blockIdx.x % a.chunks] = s;
+            a.pieces[(p.b * a.groups + p.g0 + g) * a.chunks + blockIdx.x % (unsigned)a.chunks] = s;
         } else if (q_n == 1) {
-            gm[g] = (float)s.x;
-            gr[g] = (float)rsqrt(s.y / ((double)a.spatial * (double)cg) + (double)a.eps);
+            gm[g] = s.x;
+            gr[g] = rsqrtf(__fmaf_rn(s.y, a.inv_count, a.eps));
         } else {
             gs[g] = s;
         }
@@ -181,19 +174,17 @@ __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a)
         gn_cluster_wait();
         for (int g = threadIdx.x; g < p.ng; g += nt) {
             // the CTAs' moments in rank order
-            double n = 0.0, mean = 0.0, m2 = 0.0;
+            About t;
             for (int q = 0; q < q_n; ++q) {
                 const int64_t left = a.spatial - q * a.rows;
                 if (left <= 0) break;
-                const double k = (double)(left < a.rows ? left : a.rows) * (double)cg, t = n + k;
-                const double2 s = gn_peer_f64x2(gs + g, (unsigned)q);
-                const double d = s.x - mean;
-                mean += d * (k / t);
-                m2 += s.y + d * d * (n * k / t);
-                n = t;
+                const float2 s = gn_peer_f32x2(gs + g, (unsigned)q);
+                if (q == 0) t.ref = s.x;
+                t.add((float)(left < a.rows ? left : a.rows) * (float)cg, s.x, s.y);
             }
-            gm[g] = (float)mean;
-            gr[g] = (float)rsqrt(m2 / n + (double)a.eps);
+            const float2 s = t.close();
+            gm[g] = s.x;
+            gr[g] = rsqrtf(__fmaf_rn(s.y, a.inv_count, a.eps));
         }
         gn_cluster_arrive();  // met again at the end: no CTA leaves while its moments may be read
     }
@@ -208,7 +199,7 @@ __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a)
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
         Affine<N, UNI> k;
-        k.load(col, cg, gm, gr, a.scales + p.c0, a.biases + p.c0);
+        k.load(col, cg, gm, gr, sc, bi);
         const T *src = slab + rl * p.cb + col * N;
         T *dst = y + (int64_t)rl * a.filters + (int64_t)col * N;
 #pragma unroll 2
@@ -217,8 +208,7 @@ __global__ void __launch_bounds__(512) k_gn_fwd(const __grid_constant__ GnFwd a)
             V::unpack(*reinterpret_cast<const Raw *>(src), f);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                f[i] = k.z(f[i], i);
-                f[i] = make_float2(act_quick<A>(f[i].x, a.act), act_quick<A>(f[i].y, a.act));
+                f[i] = act_pair<A>(k.z(f[i], i), a.act);
             }
             *reinterpret_cast<Raw *>(dst) = V::pack(f);
             src += rl_n * p.cb;
@@ -249,8 +239,8 @@ __global__ void __launch_bounds__(256) k_gn_merge(const __grid_constant__ GnFwd 
     for (int64_t q = lane; q < a.chunks; q += 32) {
         const int64_t left = a.spatial - q * a.rows;
         const double k = (double)(left < a.rows ? left : a.rows) * (double)a.cg;
-        const double2 piece = a.pieces[i * a.chunks + q];
-        t.add(k, piece.x, piece.y);
+        const float2 piece = a.pieces[i * a.chunks + q];
+        t.add(k, (double)piece.x, (double)piece.y);
     }
     for (int o = 16; o > 0; o >>= 1) {
         const double n = __shfl_down_sync(0xffffffffu, t.n, o), m = __shfl_down_sync(0xffffffffu, t.mean, o),
@@ -269,7 +259,7 @@ __global__ void __launch_bounds__(256) k_gn_apply(const __grid_constant__ GnFwd 
     using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
     constexpr int N = V::N, P = V::P;
-    const Place p = place_of(a, a.chunks);
+    const Place p = place_of(a, (unsigned)a.chunks);
     const int nt = blockDim.x, v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
     if (rl >= rl_n) return;
@@ -284,8 +274,7 @@ __global__ void __launch_bounds__(256) k_gn_apply(const __grid_constant__ GnFwd 
             V::unpack(*reinterpret_cast<const Raw *>(static_cast<const T *>(a.x) + at), f);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                f[i] = k.z(f[i], i);
-                f[i] = make_float2(act_quick<A>(f[i].x, a.act), act_quick<A>(f[i].y, a.act));
+                f[i] = act_pair<A>(k.z(f[i], i), a.act);
             }
             *reinterpret_cast<Raw *>(static_cast<T *>(a.y) + at) = V::pack(f);
         }
@@ -326,7 +315,7 @@ dnb_status dnb_gn_act_forward_workspace(const void *x, const void *y, int dtype,
     if (batch == 0 || spatial == 0) return DNB_OK;
     const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y);
     const GnPlan p = gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, 1, false);
-    if (p.stream) *bytes = (size_t)(batch * groups * p.chunks) * 16;
+    if (p.stream) *bytes = (size_t)(batch * groups * p.chunks) * 8;
     return DNB_OK;
 }
 
@@ -346,7 +335,7 @@ dnb_status dnb_gn_act_forward(const void *x, void *y, int dtype, int64_t batch, 
         overlaps(rstd, st, y, bytes) || overlaps(mean, st, x, bytes) || overlaps(rstd, st, x, bytes))
         return fail(DNB_ERR_INVALID, "%s: overlapping tensors", what);
     const GnPlan p = gn_plan(batch, spatial, filters, groups, e, align, 1, false);
-    const size_t need = p.stream ? (size_t)(batch * groups * p.chunks) * 16 : 0;
+    const size_t need = p.stream ? (size_t)(batch * groups * p.chunks) * 8 : 0;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(DNB_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what, need,
                     workspace ? workspace_bytes : (size_t)0);
@@ -360,7 +349,7 @@ dnb_status dnb_gn_act_forward(const void *x, void *y, int dtype, int64_t batch, 
     a.biases = biases;
     a.mean = mean;
     a.rstd = rstd;
-    a.pieces = static_cast<double2 *>(workspace);
+    a.pieces = static_cast<float2 *>(workspace);
     a.spatial = spatial;
     a.filters = filters;
     a.groups = groups;
@@ -370,8 +359,10 @@ dnb_status dnb_gn_act_forward(const void *x, void *y, int dtype, int64_t batch, 
     a.rows = p.rows;
     a.chunks = p.chunks;
     a.eps = eps;
+    a.inv_count = (float)(1.0 / ((double)spatial * (double)a.cg));
     a.act = act;
     a.cluster = p.cluster;
+    a.unit_groups = (int)(p.cb / a.cg);
     a.slab = (unsigned)p.slab;
     a.part = (unsigned)p.part;
     return dispatch_dtype(dtype, [&]<class T>() -> dnb_status {

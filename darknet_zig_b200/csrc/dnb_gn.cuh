@@ -46,6 +46,7 @@ inline dnb_status gn_shape_check(int64_t batch, int64_t spatial, int64_t filters
     if (filters % groups) return fail(DNB_ERR_INVALID, "%s: groups must divide filters", what);
     if (filters / groups > kGnMaxGroup)
         return fail(DNB_ERR_UNSUPPORTED, "%s: more than %lld channels in a group", what, (long long)kGnMaxGroup);
+    if (filters > int64_t(1) << 30) return fail(DNB_ERR_UNSUPPORTED, "%s: too many filters", what);
     const int64_t most = int64_t(1) << 44;  // elements: offsets stay far inside 63 bits
     if (filters > most || (batch && spatial && (spatial > most / filters || batch > most / filters / spatial)))
         return fail(DNB_ERR_INVALID, "%s: too large", what);
@@ -88,11 +89,12 @@ inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t g
     p.nu = (groups + per - 1) / per;
     auto sizes = [&](size_t slabs) {
         const int64_t v = p.cb / n, wide = p.threads > v ? p.threads : v;
-        // forward: two floats a thread and vector (or channel), two doubles and two floats a group;
+        // forward: two floats a thread and vector (or channel), four floats a group;
         // backward: two floats a channel of a thread, two a thread (slices), two a channel, two a group
         p.part = (size_t)(backward || !p.uni ? wide * n : wide);
         p.smem = p.slab * slabs + p.part * 8 + 64;
-        p.smem += backward ? (size_t)p.threads * 8 + (size_t)p.cb * 8 + (size_t)per * 8 : (size_t)per * 24;
+        p.smem += backward ? (size_t)p.threads * 8 + (size_t)p.cb * 8 + (size_t)per * 8 : (size_t)per * 16;
+        p.smem += (size_t)p.cb * 8;  // scales and biases
     };
     auto shape = [&](int q) {
         p.cluster = q;
@@ -122,25 +124,43 @@ inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t g
 
 // ---- device helpers ----
 
-// Where a CTA works: unit, rows, columns.
+// Where a CTA works: unit, rows, columns. (32-bit arithmetic: a 64-bit division costs a hundred instructions,
+// and a warp has a few hundred to run; gn_shape_check and gn_launch keep every count below 2^31.)
 struct Place {
     int64_t b, c0, r0;
     int nr, cb, ng, g0;
 };
 template <class Args>
-__device__ __forceinline__ Place place_of(const Args &a, int64_t per_unit) {
+__device__ __forceinline__ Place place_of(const Args &a, unsigned per_unit) {
     Place p;
-    const int64_t unit = blockIdx.x / per_unit, q = blockIdx.x % per_unit;
-    p.b = unit / a.nu;
-    p.c0 = (unit % a.nu) * a.cb;
-    p.cb = (int)(a.cb < a.filters - p.c0 ? a.cb : a.filters - p.c0);
-    p.g0 = (int)(p.c0 / a.cg);
-    p.ng = (int)(p.cb / a.cg);
-    p.r0 = q * a.rows;
+    const unsigned unit = blockIdx.x / per_unit, q = blockIdx.x - unit * per_unit;
+    const unsigned b = unit / (unsigned)a.nu, u = unit - b * (unsigned)a.nu;
+    p.b = b;
+    const int c0 = (int)u * (int)a.cb, left_c = (int)a.filters - c0;
+    p.c0 = c0;
+    p.cb = (int)a.cb < left_c ? (int)a.cb : left_c;
+    p.g0 = (int)u * a.unit_groups;
+    p.ng = (int)a.groups - p.g0 < a.unit_groups ? (int)a.groups - p.g0 : a.unit_groups;
+    p.r0 = (int64_t)q * a.rows;
     const int64_t left = a.spatial - p.r0;
     p.nr = (int)(left < 0 ? 0 : left < a.rows ? left : a.rows);
     return p;
 }
+
+// A vector from global to shared memory without passing through registers, where the hardware has such a copy
+// (16 or 4 bytes): a thread has all its rows in flight at once. gn_arrived(): the thread's own copies are there.
+template <int VB>
+__device__ __forceinline__ void gn_copy(void *dst, const void *src) {
+    if constexpr (VB == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+                     : "memory");
+    else if constexpr (VB == 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+                     : "memory");
+    else
+        *static_cast<typename RawVec<VB>::type *>(dst) = *static_cast<const typename RawVec<VB>::type *>(src);
+}
+__device__ __forceinline__ void gn_arrived() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ void gn_cluster_arrive() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -151,11 +171,6 @@ __device__ __forceinline__ uint32_t gn_peer(const void *p, unsigned rank) {
     uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
     return r;
-}
-__device__ __forceinline__ double2 gn_peer_f64x2(const void *p, unsigned rank) {
-    double2 v;
-    asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "r"(gn_peer(p, rank)) : "memory");
-    return v;
 }
 __device__ __forceinline__ float2 gn_peer_f32x2(const void *p, unsigned rank) {
     float2 v;
@@ -175,12 +190,21 @@ __device__ __forceinline__ void groups_of(int col, int cg, int (&g)[N]) {
     }
 }
 
+// The unit's scales and biases into shared memory, early: by the time they are needed their latency is over.
+__device__ __forceinline__ void gn_stage_params(float *sc, const float *scales, const float *biases, const Place &p) {
+    for (int c = threadIdx.x; c < p.cb; c += blockDim.x) {
+        sc[c] = scales[p.c0 + c];
+        sc[p.cb + c] = biases[p.c0 + c];
+    }
+}
+
 // z = (x - mean)*(rstd*scale) + bias for a vector's channels; the forward and the backward's recomputed output
 // share it, so that both see the same z.
 template <int N, bool UNI>
 struct Affine {
     static constexpr int P = (N + 1) / 2;
     float2 m[UNI ? 1 : P], k[P], b[P];
+    float rs;  // UNI: the group's rstd
     __device__ __forceinline__ void load(int col, int cg, const float *mean, const float *rstd, const float *scales,
                                          const float *biases) {
         int g[N];
@@ -188,6 +212,7 @@ struct Affine {
         const int lg = UNI ? col * N / cg : 0;
         const float um = UNI ? mean[lg] : 0.0f, ur = UNI ? rstd[lg] : 0.0f;
         if constexpr (UNI) m[0] = both(-um);
+        rs = ur;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int c = col * N + 2 * i;

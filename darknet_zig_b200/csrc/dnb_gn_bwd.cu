@@ -8,8 +8,8 @@
 // memory: x, delta (and y) in, dx out. k_gn_bwd keeps a unit (see dnb_gn.cuh) of each input in shared
 // memory: the channel sums are formed while it is loaded, dx = d*k - (x - mean)*c2 - c1 from shared memory
 // (k = rstd*scale, c1 = rstd*sum(t)/n, c2 = rstd^2*sum(t*xh)/n: two fused multiply-adds an element).
-// A channel's rows are added in fp32 per thread (rows / RL terms), across threads, CTAs and images in fp64,
-// in a fixed order; k_gn_updates adds the images up.
+// A channel's rows are added in fp32 (per thread rows / RL terms, then the threads in two steps), across CTAs,
+// images and a group's channels in fp64, in a fixed order; k_gn_updates adds the images up.
 #include "dnb_gn.cuh"
 
 namespace dnb {
@@ -23,15 +23,39 @@ struct GnBwd {
     float2 *pieces;  // streaming path: [batch][chunks][filters], the same of a row chunk
     float2 *moments; // streaming path: [batch][groups]: (sum t, sum t*xh) / n
     int64_t spatial, filters, groups, cg, cb, nu, rows, chunks;
-    int act, cluster;
+    double inv_count;  // 1 / n
+    int act, cluster, unit_groups;
     unsigned slab, part;
 };
 
-// The activation's gradient times delta, from the given output or the recomputed one (z: its argument).
+// The activation's gradient times delta for a pair, from the given output or the recomputed one (z: its
+// argument). The recomputed logistic's y(1 - y) shares one reciprocal between the two: 1/u and 1/v are v/(uv)
+// and u/(uv). Exponents are cut off at 43 (y = 2e-19) so that uv stays finite; three special-function results
+// a pair instead of four, which bound the kernel.
 template <int A, bool Y>
-__device__ __forceinline__ float through(float delta, float y, float z, int act) {
+__device__ __forceinline__ float2 through(float2 delta, float2 y, float2 z, int act) {
     if constexpr (A == DNB_ACT_LINEAR) return delta;
-    return delta * act_grad<A>(Y ? y : act_quick<A>(z, act), act);
+    if constexpr (A == DNB_ACT_LOGISTIC && !Y) {
+        float tx, ty;
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(tx) : "f"(-z.x), "f"(43.0f));
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(ty) : "f"(-z.y), "f"(43.0f));
+        const float2 e = make_float2(quick_exp(tx), quick_exp(ty)), u = __fadd2_rn(e, both(1.0f));
+        const float rcp = quick_rcp(u.x * u.y);
+        const float2 out = __fmul2_rn(both(rcp), make_float2(u.y, u.x));
+        return __fmul2_rn(delta, __fmul2_rn(__fmul2_rn(e, out), out));  // 1 - y = e y
+    }
+    const float2 o = Y ? y : act_pair<A>(z, act);
+    return make_float2(delta.x * act_grad<A>(o.x, act), delta.y * act_grad<A>(o.y, act));
+}
+
+template <int N>
+__device__ __forceinline__ void store_pairs(float *p, const float2 (&s)[(N + 1) / 2]) {
+    if constexpr (N == 1) *p = s[0].x;
+    else if constexpr (N == 2) *reinterpret_cast<float2 *>(p) = s[0];
+    else
+#pragma unroll
+        for (int i = 0; i < N / 2; i += 2)
+            *reinterpret_cast<float4 *>(p + 2 * i) = make_float4(s[i].x, s[i].y, s[i + 1].x, s[i + 1].y);
 }
 
 // The group's (c1, c2) for a vector's channels.
@@ -59,7 +83,7 @@ __device__ __forceinline__ void dx_of(float2 (&fx)[P], const float2 (&fd)[P], co
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const float2 z = Y ? fy[i] : k.z(fx[i], i);
-        const float2 d = make_float2(through<A, Y>(fd[i].x, fy[i].x, z.x, act), through<A, Y>(fd[i].y, fy[i].y, z.y, act));
+        const float2 d = through<A, Y>(fd[i], fy[i], z, act);
         const float2 xm = __fadd2_rn(fx[i], k.m[UNI ? 0 : i]);
         fx[i] = __ffma2_rn(d, k.k[i], __ffma2_rn(xm, c2[UNI ? 0 : i], c1[UNI ? 0 : i]));
     }
@@ -71,7 +95,7 @@ __global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a)
     using Raw = typename V::Raw;
     constexpr int N = V::N, P = V::P;
     extern __shared__ __align__(16) unsigned char smem[];
-    const Place p = place_of(a, STREAM ? a.chunks : a.cluster);
+    const Place p = place_of(a, STREAM ? (unsigned)a.chunks : (unsigned)a.cluster);
     T *sx = reinterpret_cast<T *>(smem), *sd = reinterpret_cast<T *>(smem + a.slab),
       *sy = reinterpret_cast<T *>(smem + 2 * a.slab);
     float *part = reinterpret_cast<float *>(smem + (STREAM ? 0u : (Y ? 3u : 2u) * a.slab));
@@ -79,6 +103,7 @@ __global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a)
     const int nt = blockDim.x;
     float2 *ch = slices + nt;                                    // the channels' sums
     float2 *mo = ch + p.cb;                                      // the groups' (c1, c2)
+    float *sc = reinterpret_cast<float *>(mo + p.ng), *bi = sc + p.cb;
     const int v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
     const bool on = rl < rl_n;
@@ -86,79 +111,107 @@ __global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a)
     const int64_t pitch = a.filters * rl_n;
     const int cg = (int)a.cg, srow = rl_n * p.cb;
 
+    gn_stage_params(sc, a.scales, a.biases, p);
+    if constexpr (!STREAM) {
+        for (int col = col0; col < v; col += vp) {
+            if (!on) break;
+            const int64_t at = base + (int64_t)rl * a.filters + (int64_t)col * N;
+            const T *x = static_cast<const T *>(a.x) + at, *delta = static_cast<const T *>(a.delta) + at;
+            const T *y = Y ? static_cast<const T *>(a.y) + at : nullptr;
+            int in = rl * p.cb + col * N;
+#pragma unroll 2
+            for (int r = rl; r < p.nr; r += rl_n) {
+                gn_copy<VB>(sx + in, x);
+                gn_copy<VB>(sd + in, delta);
+                if constexpr (Y) {
+                    gn_copy<VB>(sy + in, y);
+                    y += pitch;
+                }
+                x += pitch;
+                delta += pitch;
+                in += srow;
+            }
+        }
+    }
+    __syncthreads();
+    if constexpr (!STREAM) gn_arrived();
+
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
         Affine<N, UNI> k;
-        k.load(col, cg, a.mean + g0, a.rstd + g0, a.scales + p.c0, a.biases + p.c0);
+        k.load(col, cg, a.mean + g0, a.rstd + g0, sc, bi);
         float2 s0[P] = {}, s1[P] = {};
-        const int64_t at = base + (int64_t)rl * a.filters + (int64_t)col * N;
-        const T *x = static_cast<const T *>(a.x) + at, *delta = static_cast<const T *>(a.delta) + at;
-        const T *y = Y ? static_cast<const T *>(a.y) + at : nullptr;
-        int in = rl * p.cb + col * N;
+        const int64_t at = base + (int64_t)rl * a.filters + (int64_t)col * N, in = rl * p.cb + col * N;
+        const T *x = STREAM ? static_cast<const T *>(a.x) + at : sx + in;
+        const T *delta = STREAM ? static_cast<const T *>(a.delta) + at : sd + in;
+        const T *y = !Y ? nullptr : STREAM ? static_cast<const T *>(a.y) + at : sy + in;
+        const int64_t step = STREAM ? pitch : srow;
 #pragma unroll 2
         for (int r = rl; r < p.nr; r += rl_n) {
-            const Raw rx = *reinterpret_cast<const Raw *>(x), rd = *reinterpret_cast<const Raw *>(delta);
-            Raw ry{};
-            if constexpr (Y) {
-                ry = *reinterpret_cast<const Raw *>(y);
-                y += pitch;
-            }
-            x += pitch;
-            delta += pitch;
-            if constexpr (!STREAM) {
-                *reinterpret_cast<Raw *>(sx + in) = rx;
-                *reinterpret_cast<Raw *>(sd + in) = rd;
-                if constexpr (Y) *reinterpret_cast<Raw *>(sy + in) = ry;
-                in += srow;
-            }
             float2 fx[P], fd[P], fy[P] = {};
-            V::unpack(rx, fx);
-            V::unpack(rd, fd);
-            if constexpr (Y) V::unpack(ry, fy);
+            V::unpack(*reinterpret_cast<const Raw *>(x), fx);
+            V::unpack(*reinterpret_cast<const Raw *>(delta), fd);
+            if constexpr (Y) {
+                V::unpack(*reinterpret_cast<const Raw *>(y), fy);
+                y += step;
+            }
+            x += step;
+            delta += step;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const float2 z = Y ? fy[i] : k.z(fx[i], i);
-                const float2 d = make_float2(through<A, Y>(fd[i].x, fy[i].x, z.x, a.act),
-                                             through<A, Y>(fd[i].y, fy[i].y, z.y, a.act));
+                const float2 d = through<A, Y>(fd[i], fy[i], z, a.act);
                 s0[i] = __fadd2_rn(s0[i], d);
                 s1[i] = __ffma2_rn(d, __fadd2_rn(fx[i], k.m[UNI ? 0 : i]), s1[i]);
             }
         }
-        int g[N];
-        groups_of<N>(col, cg, g);
+        if constexpr (UNI) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            part[rl * p.cb + col * N + j] = j & 1 ? s0[j / 2].y : s0[j / 2].x;
-            part[a.part + rl * p.cb + col * N + j] = (j & 1 ? s1[j / 2].y : s1[j / 2].x) * a.rstd[g0 + g[j]];
+            for (int i = 0; i < P; ++i) s1[i] = __fmul2_rn(s1[i], both(k.rs));
+        } else {
+            int g[N];
+            groups_of<N>(col, cg, g);
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                s1[i] = __fmul2_rn(s1[i], make_float2(a.rstd[g0 + g[2 * i]], a.rstd[g0 + g[2 * i + 1 < N ? 2 * i + 1 : 0]]));
         }
+        store_pairs<N>(part + rl * p.cb + col * N, s0);
+        store_pairs<N>(part + a.part + rl * p.cb + col * N, s1);
     }
     __syncthreads();
     // a channel's sums: its row lanes in slices, one thread each, then the slices
     const int sl_n = p.cb < nt ? min(nt / p.cb, rl_n) : 1;
-    for (int t = threadIdx.x; t < p.cb * sl_n; t += nt) {
-        const int c = t % p.cb, sl = t / p.cb;
-        double s0 = 0.0, s1 = 0.0;
-        for (int r = sl; r < rl_n; r += sl_n) {
-            s0 += (double)part[r * p.cb + c];
-            s1 += (double)part[a.part + r * p.cb + c];
-        }
-        const float2 s = make_float2((float)s0, (float)s1);
-        if (sl_n == 1) ch[c] = s;
-        else slices[sl * p.cb + c] = s;
-    }
-    __syncthreads();
     if (sl_n > 1) {
-        for (int c = threadIdx.x; c < p.cb; c += nt) {
-            double s0 = 0.0, s1 = 0.0;
-            for (int sl = 0; sl < sl_n; ++sl) {
-                const float2 s = slices[sl * p.cb + c];
-                s0 += (double)s.x;
-                s1 += (double)s.y;
+        const int sl = threadIdx.x / p.cb, c = threadIdx.x - sl * p.cb;
+        if (sl < sl_n) {
+            float s0 = 0.0f, s1 = 0.0f;
+            for (int r = sl; r < rl_n; r += sl_n) {
+                s0 += part[r * p.cb + c];
+                s1 += part[a.part + r * p.cb + c];
             }
-            ch[c] = make_float2((float)s0, (float)s1);
+            slices[sl * p.cb + c] = make_float2(s0, s1);
         }
-        if (STREAM || a.cluster == 1) __syncthreads();
+        __syncthreads();
+        if (threadIdx.x < p.cb) {
+            float s0 = 0.0f, s1 = 0.0f;
+            for (int q = 0; q < sl_n; ++q) {
+                const float2 s = slices[q * p.cb + threadIdx.x];
+                s0 += s.x;
+                s1 += s.y;
+            }
+            ch[threadIdx.x] = make_float2(s0, s1);
+        }
+    } else {
+        for (int c = threadIdx.x; c < p.cb; c += nt) {
+            float s0 = 0.0f, s1 = 0.0f;
+            for (int r = 0; r < rl_n; ++r) {
+                s0 += part[r * p.cb + c];
+                s1 += part[a.part + r * p.cb + c];
+            }
+            ch[c] = make_float2(s0, s1);
+        }
     }
+    if (STREAM || a.cluster == 1) __syncthreads();
     if constexpr (STREAM) {
         for (int c = threadIdx.x; c < p.cb; c += nt)
             a.pieces[(p.b * a.chunks + blockIdx.x % a.chunks) * a.filters + p.c0 + c] = ch[c];
@@ -184,20 +237,19 @@ __global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a)
     }
     if (p.r0 == 0)
         for (int c = threadIdx.x; c < p.cb; c += nt) a.image[p.b * a.filters + p.c0 + c] = all[c];
-    const double count = (double)a.spatial * (double)a.cg;
     const int lane = threadIdx.x & 31;
     for (int g = threadIdx.x >> 5; g < p.ng; g += nt >> 5) {
         double s0 = 0.0, s1 = 0.0;
         for (int c = lane; c < cg; c += 32) {
-            const double sc = (double)a.scales[p.c0 + g * cg + c];
-            s0 += sc * (double)all[g * cg + c].x;
-            s1 += sc * (double)all[g * cg + c].y;
+            const double by = (double)sc[g * cg + c];
+            s0 += by * (double)all[g * cg + c].x;
+            s1 += by * (double)all[g * cg + c].y;
         }
         s0 = warp_sum(s0);
         s1 = warp_sum(s1);
         if (lane == 0) {
             const double rs = (double)a.rstd[g0 + g];
-            mo[g] = make_float2((float)(-rs * s0 / count), (float)(-rs * rs * s1 / count));
+            mo[g] = make_float2((float)(-rs * s0 * a.inv_count), (float)(-rs * rs * s1 * a.inv_count));
         }
     }
     __syncthreads();
@@ -205,7 +257,7 @@ __global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a)
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
         Affine<N, UNI> k;
-        k.load(col, cg, a.mean + g0, a.rstd + g0, a.scales + p.c0, a.biases + p.c0);
+        k.load(col, cg, a.mean + g0, a.rstd + g0, sc, bi);
         float2 c1[UNI ? 1 : P], c2[UNI ? 1 : P];
         load_moments<N, UNI>(col, cg, mo, c1, c2);
         T *dx = static_cast<T *>(a.dx) + base + (int64_t)rl * a.filters + (int64_t)col * N;
@@ -251,11 +303,10 @@ __global__ void __launch_bounds__(128) k_gn_bwd_merge(const __grid_constant__ Gn
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        const double n = (double)a.spatial * (double)a.cg;
         t0 = red[0][0] + red[0][1] + red[0][2] + red[0][3];
         t1 = red[1][0] + red[1][1] + red[1][2] + red[1][3];
         const double rs = (double)a.rstd[blockIdx.x];
-        a.moments[blockIdx.x] = make_float2((float)(-rs * t0 / n), (float)(-rs * rs * t1 / n));
+        a.moments[blockIdx.x] = make_float2((float)(-rs * t0 * a.inv_count), (float)(-rs * rs * t1 * a.inv_count));
     }
 }
 
@@ -264,7 +315,7 @@ __global__ void __launch_bounds__(256) k_gn_bwd_apply(const __grid_constant__ Gn
     using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
     constexpr int N = V::N, P = V::P;
-    const Place p = place_of(a, a.chunks);
+    const Place p = place_of(a, (unsigned)a.chunks);
     const int nt = blockDim.x, v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
     if (rl >= rl_n) return;
@@ -429,8 +480,10 @@ dnb_status dnb_gn_act_backward(const void *x, const void *y, const void *delta, 
     a.nu = p.nu;
     a.rows = p.rows;
     a.chunks = p.chunks;
+    a.inv_count = 1.0 / ((double)spatial * (double)a.cg);
     a.act = act;
     a.cluster = p.cluster;
+    a.unit_groups = (int)(p.cb / a.cg);
     a.slab = (unsigned)p.slab;
     a.part = (unsigned)p.part;
     auto with_y = [&]<class T, int VB, int A, bool UNI>() {

@@ -141,14 +141,33 @@ struct Pairs {
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
 
+// The special-function unit's exponential and reciprocal, subnormals flushed (no scaling around them).
+__device__ __forceinline__ float quick_exp(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+__device__ __forceinline__ float quick_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // An activation of the 16-bit entries: the fp32 entries' (dnb_common.cuh), but for the logistic, whose
 // exponential and reciprocal are the special-function unit's (2 ulp each; a division and an exponential to
 // the last bit cost a third of a group norm's time and vanish in the rounding to 16 bits).
 template <int A>
 __device__ __forceinline__ float act_quick(float x, int a) {
-    if constexpr (A == DNB_ACT_LOGISTIC) return __fdividef(1.0f, 1.0f + __expf(-x));
-    else if constexpr (A == DNB_ACT_LEAKY) return fmaxf(x, 0.1f * x);
+    if constexpr (A == DNB_ACT_LOGISTIC) return quick_rcp(1.0f + quick_exp(-x));
     else return act_fwd<A>(x, a);
+}
+template <int A>
+__device__ __forceinline__ float2 act_pair(float2 x, int a) {
+    if constexpr (A == DNB_ACT_LEAKY) {  // the larger of x and 0.1 x (fmaxf of two NaNs is NaN)
+        const float2 t = __fmul2_rn(x, both(0.1f));
+        return make_float2(fmaxf(x.x, t.x), fmaxf(x.y, t.y));
+    }
+    return make_float2(act_quick<A>(x.x, a), act_quick<A>(x.y, a));
 }
 
 // Calls f.template operator()<T>() with the element type.
