@@ -59,6 +59,7 @@ class DnbError(RuntimeError):
         super().__init__(f"{what}: {detail or 'status %d' % status}")
 
 
+_bound: dict[str, tuple] = {}  # entry points called so far: (function, argument count)
 _lock = threading.Lock()
 _lib = None
 _sigs = None
@@ -92,12 +93,16 @@ def call(name: str, *args) -> None:
     """Calls dnb_<name>(*args) and raises DnbError on a non-zero status. The argument count
     must match the header's: ctypes would convert surplus arguments by guesswork (a pointer
     passed as a C int is truncated) instead of refusing them."""
-    L = lib()
-    fn = getattr(L, "dnb_" + name)
-    if len(args) != len(fn.argtypes):
-        raise TypeError(f"dnb_{name} takes {len(fn.argtypes)} arguments, {len(args)} given")
+    bound = _bound.get(name)
+    if bound is None:
+        fn = getattr(lib(), "dnb_" + name)
+        bound = _bound[name] = (fn, len(fn.argtypes))
+    fn, n = bound
+    if len(args) != n:
+        raise TypeError(f"dnb_{name} takes {n} arguments, {len(args)} given")
     st = fn(*args)
     if st != 0:
+        L = lib()
         detail = L.dnb_last_error_detail()
         detail = detail.decode() if detail else ""
         err = L.dnb_error_string(st)

@@ -219,14 +219,9 @@ dnb_status dnb_connected_act_forward(const void *x, int64_t ldx, const void *w, 
         });
     }
     Operand a{x, ldx}, b{w, ldw};
-    if (f.x) {
-        DNB_TRY(pack_rows(x, ldx, f.x, batch, inputs, dtype, {}, ds, s, what));
-        a = {f.x, packed_ld(inputs)};
-    }
-    if (f.w) {
-        DNB_TRY(pack_rows(w, ldw, f.w, outputs, inputs, dtype, {}, ds, s, what));
-        b = {f.w, packed_ld(inputs)};
-    }
+    DNB_TRY(pack_rows({x, ldx, f.x, batch, inputs}, {w, ldw, f.w, outputs, inputs}, dtype, {}, ds, s, what));
+    if (f.x) a = {f.x, packed_ld(inputs)};
+    if (f.w) b = {f.w, packed_ld(inputs)};
     EpiOut e = epilogue(y, ldy, dtype, batch, outputs);
     e.bias = biases;
     e.act = act;
@@ -346,12 +341,11 @@ dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w,
     if (inputs == 0) return DNB_OK;
     Operand d{linear ? delta : dz, linear ? ldd : lddz};
     if (f.dz) d = {f.dz, packed_ld(outputs)};
+    DNB_TRY(pack_rows({x, ldx, weight_updates ? f.x : nullptr, batch, inputs},
+                      {w, ldw, dx ? f.w : nullptr, outputs, inputs}, dtype, {}, ds, s, what));
     if (dx) {
         Operand b{w, ldw};
-        if (f.w) {
-            DNB_TRY(pack_rows(w, ldw, f.w, outputs, inputs, dtype, {}, ds, s, what));
-            b = {f.w, packed_ld(inputs)};
-        }
+        if (f.w) b = {f.w, packed_ld(inputs)};
         EpiOut e = epilogue(dx, lddx, dtype, batch, inputs);
         if (add_x) add_to(e, dx, lddx, dtype);
         const dnb_status st = product<false, true>(d, b, dtype, batch, inputs, outputs, e, ds, s, what);
@@ -359,10 +353,7 @@ dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w,
     }
     if (weight_updates) {
         Operand b{x, ldx};
-        if (f.x) {
-            DNB_TRY(pack_rows(x, ldx, f.x, batch, inputs, dtype, {}, ds, s, what));
-            b = {f.x, packed_ld(inputs)};
-        }
+        if (f.x) b = {f.x, packed_ld(inputs)};
         EpiOut e = epilogue(weight_updates, lddw, updates_dtype, outputs, inputs);
         if (add_w) add_to(e, weight_updates, lddw, updates_dtype);
         const dnb_status st = product<true, true>(d, b, dtype, outputs, inputs, batch, e, ds, s, what);

@@ -24,20 +24,39 @@ EncodeFn encoder() {
     return fn;
 }
 
-// Eight elements a thread: 16-byte stores whatever the source's alignment.
+// Eight elements a thread: 16-byte stores whatever the source's alignment. Vectors [0, split) are job 0's, the
+// rest job 1's, so that a product's two operands take one launch.
 template <class T>
-__global__ void __launch_bounds__(256) k_pack(const T *src, int64_t lds, T *dst, int64_t ldd, int64_t rows,
-                                              int64_t cols, int64_t per, Gather g) {
-    const int64_t kept = g.count ? *g.count : rows, end = g.count ? (kept + 63) / 64 * 64 : rows;
-    const int64_t total = end * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per, c = (i - r * per) * 8;
-        uint4 out = make_uint4(0u, 0u, 0u, 0u);
-        if (r < kept) {
-            const int64_t at = g.rows ? g.rows[r] : r;
-            const T *p = src + at * lds + c;
-            typename Vec<T, 16>::U u;
-            u.raw = out;
+struct PackArgs {
+    const T *src[2];
+    T *dst[2];
+    int64_t lds[2], ldd[2], rows[2], cols[2], per[2], split;
+    FastDiv div[2];  // by per, where the job's vectors are below 2^32
+    Gather g;        // job 0's
+};
+template <class T>
+__global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackArgs<T> a) {
+    const int64_t kept = a.g.count ? *a.g.count : a.rows[0], end = a.g.count ? (kept + 63) / 64 * 64 : a.rows[0];
+    const int64_t total = a.split + a.rows[1] * a.per[1];
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+        const int job = at >= a.split;
+        const int64_t i = job ? at - a.split : at, per = a.per[job];
+        int64_t r, c;
+        if (a.rows[job] * per <= 0xffffffc0ll) {
+            uint32_t q, m;
+            a.div[job].divmod((uint32_t)i, q, m);
+            r = q;
+            c = (int64_t)m * 8;
+        } else {
+            r = i / per;
+            c = (i - r * per) * 8;
+        }
+        typename Vec<T, 16>::U u;
+        u.raw = make_uint4(0u, 0u, 0u, 0u);
+        if (job == 0 && r >= end) continue;
+        if (job == 1 || r < kept) {
+            const int64_t from = job == 0 && a.g.rows ? a.g.rows[r] : r, cols = a.cols[job];
+            const T *p = a.src[job] + from * a.lds[job] + c;
             if (c + 8 <= cols && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
                 u.raw = *reinterpret_cast<const uint4 *>(p);
             } else {
@@ -45,17 +64,16 @@ __global__ void __launch_bounds__(256) k_pack(const T *src, int64_t lds, T *dst,
                 for (int j = 0; j < 8; ++j)
                     if (c + j < cols) u.e[j] = p[j];
             }
-            if (g.factor) {
+            if (job == 0 && a.g.factor) {
                 float f[8];
                 Vec<T, 16>::unpack(u.raw, f);
-                const float by = g.factor[at] * *g.norm;
+                const float by = a.g.factor[from] * *a.g.norm;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) f[j] *= by;
                 u.raw = Vec<T, 16>::pack(f);
             }
-            out = u.raw;
         }
-        *reinterpret_cast<uint4 *>(dst + r * ldd + c) = out;
+        *reinterpret_cast<uint4 *>(a.dst[job] + r * a.ldd[job] + c) = u.raw;
     }
 }
 
@@ -111,13 +129,29 @@ dnb_status make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t oute
     return DNB_OK;
 }
 
-dnb_status pack_rows(const void *src, int64_t lds, void *dst, int64_t rows, int64_t cols, int dtype, const Gather &g,
-                     const DeviceState *ds, cudaStream_t s, const char *what) {
-    const int64_t per = (cols + 7) / 8, out_rows = g.count ? (rows + 63) / 64 * 64 : rows;
-    return dispatch_dtype16(dtype, [&]<class T>() {
-        k_pack<T><<<grid_for(out_rows * per, 256, ds), 256, 0, s>>>(static_cast<const T *>(src), lds,
-                                                                    static_cast<T *>(dst), packed_ld(cols), rows, cols,
-                                                                    per, g);
+dnb_status pack_rows(const PackJob &x, const PackJob &w, int dtype, const Gather &g, const DeviceState *ds,
+                     cudaStream_t s, const char *what) {
+    return dispatch_dtype16(dtype, [&]<class T>() -> dnb_status {
+        PackArgs<T> a{};
+        const PackJob *jobs[2] = {&x, &w};
+        int64_t vectors[2];
+        for (int k = 0; k < 2; ++k) {
+            const PackJob &q = *jobs[k];
+            a.src[k] = static_cast<const T *>(q.src);
+            a.dst[k] = static_cast<T *>(q.dst);
+            a.lds[k] = q.ld;
+            a.ldd[k] = packed_ld(q.cols);
+            a.rows[k] = q.dst ? q.rows : 0;
+            if (k == 0 && g.count) a.rows[k] = (a.rows[k] + 63) / 64 * 64;
+            a.cols[k] = q.cols;
+            a.per[k] = q.dst ? (q.cols + 7) / 8 : 1;
+            a.div[k] = FastDiv((uint32_t)a.per[k]);
+            vectors[k] = a.rows[k] * a.per[k];
+        }
+        if (vectors[0] + vectors[1] == 0) return DNB_OK;
+        a.split = vectors[0];
+        a.g = g;
+        k_pack<T><<<grid_for(vectors[0] + vectors[1], 256, ds), 256, 0, s>>>(a);
         return after_launch(s, what);
     });
 }

@@ -262,11 +262,14 @@ __global__ void __launch_bounds__(256) k_gn_apply(const __grid_constant__ GnFwd 
     const Place p = place_of(a, (unsigned)a.chunks);
     const int nt = blockDim.x, v = p.cb / N, vp = v < nt ? v : nt, rl_n = v < nt ? nt / v : 1;
     const int col0 = threadIdx.x % vp, rl = threadIdx.x / vp;
+    extern __shared__ __align__(16) float params[];
+    gn_stage_params(params, a.scales, a.biases, p);
+    __syncthreads();
     if (rl >= rl_n) return;
     const int64_t base = (p.b * a.spatial + p.r0) * a.filters + p.c0, g0 = p.b * a.groups + p.g0;
     for (int col = col0; col < v; col += vp) {
         Affine<N, UNI> k;
-        k.load(col, (int)a.cg, a.mean + g0, a.rstd + g0, a.scales + p.c0, a.biases + p.c0);
+        k.load(col, (int)a.cg, a.mean + g0, a.rstd + g0, params, params + p.cb);
 #pragma unroll 4
         for (int r = rl; r < p.nr; r += rl_n) {
             const int64_t at = base + (int64_t)r * a.filters + (int64_t)col * N;
@@ -291,7 +294,7 @@ dnb_status run_fwd(GnFwd a, const GnPlan &p, int64_t batch, const DeviceState *d
     const int64_t total = batch * a.groups;
     k_gn_merge<<<(unsigned)((total + 7) / 8), 256, 0, s>>>(a, total);
     DNB_TRY(after_launch(s, what));
-    k_gn_apply<T, VB, A, UNI><<<(unsigned)(units * p.chunks), p.threads, 0, s>>>(a);
+    k_gn_apply<T, VB, A, UNI><<<(unsigned)(units * p.chunks), p.threads, (size_t)p.cb * 8, s>>>(a);
     return after_launch(s, what);
 }
 

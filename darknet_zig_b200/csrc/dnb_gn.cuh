@@ -34,7 +34,7 @@ struct GnPlan {
     size_t smem = 0;
 };
 
-constexpr size_t kGnSmemTarget = 100 * 1024;  // two CTAs an SM
+constexpr size_t kGnSmemTarget = 112 * 1024;  // two CTAs an SM
 constexpr size_t kGnSmemMax = 200 * 1024;
 constexpr size_t kGnStreamBytes = 64 * 1024;  // a streaming chunk's inputs
 constexpr int kGnMaxCluster = 8;
@@ -62,7 +62,9 @@ inline int64_t gcd64(int64_t a, int64_t b) {
     return a;
 }
 
-// tensors: inputs held in shared memory (1 forward, 2 or 3 backward); align: the OR of the tensors' addresses.
+// tensors: planes of vectors held in shared memory (1 forward, 2 or 3 backward); align: the OR of the tensors'
+// addresses. Whether a unit streams, and how, does not depend on `tensors`: the backward's workspace is asked for
+// before its activation is known.
 inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t groups, int64_t esize, uintptr_t align,
                       int tensors, bool backward) {
     constexpr int sms = 148;  // a B200's; the plan must not depend on the current device, for the workspace's size
@@ -80,36 +82,37 @@ inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t g
     auto slab_of = [&](int64_t g, int64_t rows) { return (size_t)((rows * g * cg * esize + 15) / 16 * 16); };
     auto units_of = [&](int64_t g) { return batch * ((groups + g - 1) / g); };
     // short planes: wider units, while they still fill the SMs twice
-    while (per < groups && cap(2 * per) * cg <= 2048 && slab_of(cap(2 * per), spatial) * tensors <= 16 * 1024 &&
+    while (per < groups && cap(2 * per) * cg <= 2048 && slab_of(cap(2 * per), spatial) <= (backward ? 8 : 16) * 1024 &&
            units_of(cap(2 * per)) >= 2 * sms)
         per = cap(2 * per);
     // rows narrower than 64 bytes rather than a second read of the inputs
-    if (slab_of(per, (spatial + kGnMaxCluster - 1) / kGnMaxCluster) * tensors > kGnSmemMax && step < per) per = cap(step);
+    const int most_planes = backward ? 3 : 1;
+    if (slab_of(per, (spatial + kGnMaxCluster - 1) / kGnMaxCluster) * most_planes > kGnSmemMax && step < per)
+        per = cap(step);
     p.cb = per * cg;
     p.nu = (groups + per - 1) / per;
     auto sizes = [&](size_t slabs) {
         const int64_t v = p.cb / n, wide = p.threads > v ? p.threads : v;
         // forward: two floats a thread and vector (or channel), four floats a group;
         // backward: two floats a channel of a thread, two a thread (slices), two a channel, two a group
-        p.part = (size_t)(backward || !p.uni ? wide * n : wide);
+        p.part = (size_t)(((backward || !p.uni ? wide * n : wide) + 3) / 4 * 4);
         p.smem = p.slab * slabs + p.part * 8 + 64;
         p.smem += backward ? (size_t)p.threads * 8 + (size_t)p.cb * 8 + (size_t)per * 8 : (size_t)per * 16;
         p.smem += (size_t)p.cb * 8;  // scales and biases
     };
-    auto shape = [&](int q) {
+    auto shape = [&](int q, int planes) {
         p.cluster = q;
         p.rows = (spatial + q - 1) / q;
         p.slab = slab_of(per, p.rows);
-        p.threads = p.slab * tensors > 64 * 1024 ? 512 : 256;
-        sizes((size_t)tensors);
+        // a warp's fixed work (places, reductions) is that of a dozen vectors: no more threads than get those
+        p.threads = p.rows * (p.cb / n) >= 12 * 512 ? 512 : 256;
+        sizes((size_t)planes);
     };
-    int q = 1;
-    shape(q);
-    while (q < kGnMaxCluster && p.smem > kGnSmemTarget) shape(q *= 2);
+    shape(kGnMaxCluster, most_planes);
     if (p.smem > kGnSmemMax) {
         p.stream = true;
         p.cluster = 1;
-        p.rows = (int64_t)(kGnStreamBytes / (size_t)(p.cb * esize * tensors));
+        p.rows = (int64_t)(kGnStreamBytes / (size_t)(p.cb * esize * (backward ? 2 : 1)));
         if (p.rows < 1) p.rows = 1;
         p.chunks = (spatial + p.rows - 1) / p.rows;
         p.slab = 0;
@@ -117,8 +120,11 @@ inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t g
         sizes(0);
         return p;
     }
+    int q = 1;
+    shape(q, tensors);
+    while (q < kGnMaxCluster && p.smem > kGnSmemTarget) shape(q *= 2, tensors);
     // few units: more CTAs for each, while a CTA keeps 8 KB
-    while (q < kGnMaxCluster && units_of(per) * q < sms && p.slab * tensors > 16 * 1024) shape(q *= 2);
+    while (q < kGnMaxCluster && units_of(per) * q < sms && p.slab * tensors > 16 * 1024) shape(q *= 2, tensors);
     return p;
 }
 
@@ -198,6 +204,25 @@ __device__ __forceinline__ void gn_stage_params(float *sc, const float *scales, 
     }
 }
 
+// N consecutive floats as pairs, in the widest accesses the alignment of p allows for every N (16 bytes from
+// N = 4 on: the units start on whole vectors). From global memory one by one (the caller's vectors are
+// aligned to their element alone).
+template <int N>
+__device__ __forceinline__ void load_pairs(const float *p, float2 (&f)[(N + 1) / 2]) {
+    if constexpr (N == 1) {
+        f[0] = make_float2(*p, 0.0f);
+    } else if constexpr (N == 2) {
+        f[0] = *reinterpret_cast<const float2 *>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; i += 2) {
+            const float4 v = *reinterpret_cast<const float4 *>(p + 2 * i);
+            f[i] = make_float2(v.x, v.y);
+            f[i + 1] = make_float2(v.z, v.w);
+        }
+    }
+}
+
 // z = (x - mean)*(rstd*scale) + bias for a vector's channels; the forward and the backward's recomputed output
 // share it, so that both see the same z.
 template <int N, bool UNI>
@@ -213,14 +238,13 @@ struct Affine {
         const float um = UNI ? mean[lg] : 0.0f, ur = UNI ? rstd[lg] : 0.0f;
         if constexpr (UNI) m[0] = both(-um);
         rs = ur;
+        load_pairs<N>(scales + col * N, k);
+        load_pairs<N>(biases + col * N, b);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int c = col * N + 2 * i;
             const bool two = 2 * i + 1 < N;
             if constexpr (!UNI) m[i] = make_float2(-mean[g[2 * i]], two ? -mean[g[two ? 2 * i + 1 : 0]] : 0.0f);
-            k[i] = make_float2((UNI ? ur : rstd[g[2 * i]]) * scales[c],
-                               two ? (UNI ? ur : rstd[g[two ? 2 * i + 1 : 0]]) * scales[c + 1] : 0.0f);
-            b[i] = make_float2(biases[c], two ? biases[c + 1] : 0.0f);
+            k[i] = __fmul2_rn(k[i], UNI ? both(ur) : make_float2(rstd[g[2 * i]], two ? rstd[g[two ? 2 * i + 1 : 0]] : 0.0f));
         }
     }
     __device__ __forceinline__ float2 z(float2 x, int i) const {

@@ -8,15 +8,21 @@ namespace dnb {
 inline int64_t packed_ld(int64_t cols) { return (cols + 7) / 8 * 8; }
 inline int64_t packed_bytes(int64_t rows, int64_t cols) { return rows * packed_ld(cols) * 2; }
 
-// Copies a matrix to rows packed_ld(cols) apart at a 16-byte aligned dst. With a row map, the map's first
-// *count rows are gathered, and zero rows follow up to a multiple of 64. With factors, row r of the source is
-// multiplied by factor[r] * *norm and rounded again. dnb_gemm.cu.
+// Copies up to two matrices to rows packed_ld(cols) apart at 16-byte aligned dst, in one launch (dst NULL: none).
+// With a row map, the first matrix's rows are the map's first *count, gathered, with zero rows after them up to
+// a multiple of 64. With factors, row r of it is multiplied by factor[r] * *norm and rounded again. dnb_gemm.cu.
+struct PackJob {
+    const void *src = nullptr;
+    int64_t ld = 0;
+    void *dst = nullptr;
+    int64_t rows = 0, cols = 0;
+};
 struct Gather {
     const int *rows = nullptr, *count = nullptr;
     const float *factor = nullptr, *norm = nullptr;
 };
-dnb_status pack_rows(const void *src, int64_t lds, void *dst, int64_t rows, int64_t cols, int dtype, const Gather &g,
-                     const DeviceState *ds, cudaStream_t s, const char *what);
+dnb_status pack_rows(const PackJob &x, const PackJob &w, int dtype, const Gather &g, const DeviceState *ds,
+                     cudaStream_t s, const char *what);
 
 inline dnb_status product_shape_check(int dtype, int64_t m, int64_t k, int64_t n, const char *what) {
     if (!valid_dtype16(dtype)) return fail(DNB_ERR_INVALID, "%s: dtype must be bf16 or f16", what);

@@ -91,20 +91,19 @@ template <class T, int VB>
 struct Pairs {
     static constexpr int N = VB / (int)sizeof(T), P = (N + 1) / 2;
     using Raw = typename RawVec<VB>::type;
-    static __device__ __forceinline__ void unpack(const Raw &raw, float2 (&f)[P]) {
+    // by value: a reference would be read word by word from where it points to
+    static __device__ __forceinline__ void unpack(Raw raw, float2 (&f)[P]) {
         if constexpr (N == 1) {
             float v[1];
             Vec<T, VB>::unpack(raw, v);
             f[0] = make_float2(v[0], 0.0f);
         } else if constexpr (sizeof(T) == 4) {
-            float v[N];
-            Vec<T, VB>::unpack(raw, v);
 #pragma unroll
-            for (int i = 0; i < P; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+            for (int i = 0; i < P; ++i)
+                f[i] = make_float2(__uint_as_float(word_of(raw, 2 * i)), __uint_as_float(word_of(raw, 2 * i + 1)));
         } else {
-            const uint32_t *w = reinterpret_cast<const uint32_t *>(&raw);
 #pragma unroll
-            for (int i = 0; i < P; ++i) f[i] = pair(w[i], static_cast<T *>(nullptr));
+            for (int i = 0; i < P; ++i) f[i] = pair(word_of(raw, i), static_cast<T *>(nullptr));
         }
     }
     static __device__ __forceinline__ Raw pack(const float2 (&f)[P]) {
@@ -114,13 +113,20 @@ struct Pairs {
         if constexpr (N == 1 || sizeof(T) == 4) {
             return Vec<T, VB>::pack(v);
         } else {
-            Raw raw;
-            uint32_t *w = reinterpret_cast<uint32_t *>(&raw);
+            uint32_t w[P];
 #pragma unroll
             for (int i = 0; i < P; ++i) w[i] = word(f[i], static_cast<T *>(nullptr));
-            return raw;
+            if constexpr (P == 4) return make_uint4(w[0], w[1], w[2], w[3]);
+            else if constexpr (P == 2) return make_uint2(w[0], w[1]);
+            else return w[0];
         }
     }
+    static __device__ __forceinline__ uint32_t word_of(uint4 r, int i) {
+        return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w;
+    }
+    static __device__ __forceinline__ uint32_t word_of(uint2 r, int i) { return i == 0 ? r.x : r.y; }
+    static __device__ __forceinline__ uint32_t word_of(uint32_t r, int) { return r; }
+    static __device__ __forceinline__ uint32_t word_of(uint16_t r, int) { return r; }
     static __device__ __forceinline__ float2 pair(uint32_t w, __nv_bfloat16 *) {
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     }

@@ -395,17 +395,12 @@ dnb_status dnb_connected_xent_forward(const void *x, int64_t ldx, const void *w,
         k_kept_rows<<<1, 1024, 0, s>>>(labels, batch, classes, f.rows, f.count, nullptr, 1.0f, nullptr);
         DNB_TRY(after_launch(s, what));
     }
-    if (f.x) {
-        Gather g;
-        g.rows = f.rows;
-        g.count = f.count;
-        DNB_TRY(pack_rows(x, ldx, f.x, batch, inputs, dtype, g, ds, s, what));
-        a = {f.x, packed_ld(inputs)};
-    }
-    if (f.w) {
-        DNB_TRY(pack_rows(w, ldw, f.w, classes, inputs, dtype, {}, ds, s, what));
-        b = {f.w, packed_ld(inputs)};
-    }
+    Gather g;
+    g.rows = f.rows;
+    g.count = f.count;
+    DNB_TRY(pack_rows({x, ldx, f.x, batch, inputs}, {w, ldw, f.w, classes, inputs}, dtype, g, ds, s, what));
+    if (f.x) a = {f.x, packed_ld(inputs)};
+    if (f.w) b = {f.w, packed_ld(inputs)};
     EpiStats e{biases, labels, f.rows, f.count, f.part, f.at_label, batch, classes, f.bn};
     const dnb_status st =
         f.bn == 256
@@ -485,19 +480,16 @@ dnb_status dnb_connected_xent_backward(const void *x, int64_t ldx, const void *w
     Gather g;
     g.rows = f.rows;
     g.count = f.count;
-    DNB_TRY(pack_rows(x, ldx, f.x, batch, inputs, dtype, g, ds, s, what));
+    DNB_TRY(pack_rows({x, ldx, f.x, batch, inputs}, {w, ldw, f.w, classes, inputs}, dtype, g, ds, s, what));
     const Operand xp{f.x, packed_ld(inputs)};
     Operand xs = xp, wp{w, ldw};
     if (weight_updates && row_scales) {
         g.factor = row_scales;
         g.norm = f.meta;
-        DNB_TRY(pack_rows(x, ldx, f.xs, batch, inputs, dtype, g, ds, s, what));
+        DNB_TRY(pack_rows({x, ldx, f.xs, batch, inputs}, {}, dtype, g, ds, s, what));
         xs.p = f.xs;
     }
-    if (f.w) {
-        DNB_TRY(pack_rows(w, ldw, f.w, classes, inputs, dtype, {}, ds, s, what));
-        wp = {f.w, packed_ld(inputs)};
-    }
+    if (f.w) wp = {f.w, packed_ld(inputs)};
     if (dx && !add_x) DNB_TRY(zero_rows(dx, batch, inputs, lddx, 2, ds, s, what, labels, classes));
     const int64_t rows = (batch + 63) / 64 * 64;
     for (int64_t p = 0; p < f.pieces; ++p) {

@@ -36,7 +36,9 @@ def _p(t, dtype=torch.float32):
 
 
 def _s():
-    return torch.cuda.current_stream().cuda_stream
+    """The handle of torch's current stream (without the Stream object that torch.cuda.current_stream() makes:
+    3 us of a small op's 8)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 # ---- device / memory (gpu.zig:259-410) --------------------------------------------------
@@ -265,11 +267,13 @@ DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 ACC_UPDATES, ACC_DELTA = 1, 2
 
 
-def _on_device(t, name):
+def _refuse(t, name, want):
+    """Why a tensor argument is refused."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name}: expected a CUDA tensor")
-    if t.device.index != torch.cuda.current_device():
+        raise TypeError(f"{name}: expected a CUDA tensor, got {type(t).__name__}")
+    if t.get_device() != torch.cuda.current_device():
         raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    raise ValueError(f"{name}: expected {want}, got {tuple(t.shape)} {t.dtype} with strides {t.stride()}")
 
 
 def _dtype(t, name, allowed=(torch.bfloat16, torch.float16)):
@@ -279,13 +283,13 @@ def _dtype(t, name, allowed=(torch.bfloat16, torch.float16)):
 
 
 def _vec(t, name, n, dtype=torch.float32, optional=False):
-    """Pointer of a contiguous vector of n elements."""
+    """Pointer of n contiguous elements on the current device."""
     if t is None and optional:
         return None
-    _on_device(t, name)
-    if t.dtype != dtype or not t.is_contiguous() or t.numel() != n:
-        raise ValueError(f"{name}: expected {n} contiguous {dtype} elements, got {tuple(t.shape)} {t.dtype}")
-    return t.data_ptr()
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.numel() == n and t.is_contiguous()
+            and t.get_device() == torch._C._cuda_getDevice()):
+        return t.data_ptr()
+    return _refuse(t, name, f"{n} contiguous {dtype} elements")
 
 
 def _mat(t, name, rows, cols, dtype, optional=False):
@@ -293,16 +297,15 @@ def _mat(t, name, rows, cols, dtype, optional=False):
     tensor of rows * cols elements."""
     if t is None and optional:
         return None, cols
-    _on_device(t, name)
-    if t.dtype != dtype:
-        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols and (t.stride(1) == 1 or cols <= 1) and (
-            rows <= 1 or t.stride(0) >= cols):
-        return t.data_ptr(), max(t.stride(0), cols) if rows > 1 else cols
-    if t.is_contiguous() and t.numel() == rows * cols:
-        return t.data_ptr(), cols
-    raise ValueError(f"{name}: expected a [{rows}, {cols}] matrix with contiguous rows, got {tuple(t.shape)} with "
-                     f"strides {t.stride()}")
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == torch._C._cuda_getDevice():
+        if t.is_contiguous():
+            if t.numel() == rows * cols:
+                return t.data_ptr(), cols
+        elif t.dim() == 2 and t.shape == (rows, cols):
+            ld, one = t.stride()
+            if (one == 1 or cols <= 1) and (rows <= 1 or ld >= cols):
+                return t.data_ptr(), ld if rows > 1 else cols
+    return _refuse(t, name, f"a [{rows}, {cols}] matrix of {dtype} with contiguous rows")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -321,10 +324,7 @@ def _workspace(workspace, name, *args):
     """(pointer, bytes) of the given workspace or of one that torch allocates, with the tensor that holds it.
     The caller keeps the tensor until the launch; torch orders its reuse on the current stream."""
     if workspace is not None:
-        _on_device(workspace, "workspace")
-        if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-            raise TypeError("workspace: expected a contiguous uint8 tensor")
-        return workspace.data_ptr(), workspace.numel(), workspace
+        return _vec(workspace, "workspace", workspace.numel(), torch.uint8), workspace.numel(), workspace
     n = _workspace_bytes(name, args)
     if n == 0:
         return None, 0, None
