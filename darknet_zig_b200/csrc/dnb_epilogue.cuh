@@ -5,6 +5,23 @@
 
 namespace dnb {
 
+__device__ __forceinline__ void store32(uint4 *p, uint4 a, uint4 b) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+// A tile's biases from shared memory (the same address in every lane).
+__device__ __forceinline__ void add_bias32(float (&v)[32], const float *bias) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        const float4 b = *reinterpret_cast<const float4 *>(bias + j);
+        v[j] += b.x;
+        v[j + 1] += b.y;
+        v[j + 2] += b.z;
+        v[j + 3] += b.w;
+    }
+}
+
 // out = act(f * acc + bias[n] + add[m][n]) (add may be out), f = alpha * *alpha_dev * row_factor[row].
 // With a row map, row r of the product is row rows[r] of out, add and row_factor. A thread holds 32 columns
 // of a row: 64 contiguous bytes of 16-bit output, 128 of fp32, so its accesses fill whole sectors.
@@ -22,6 +39,8 @@ struct EpiOut {
     int act = DNB_ACT_LINEAR;
     int64_t m = 0, n = 0;
     bool vec_out = false, vec_add = false;  // rows start on 16-byte boundaries
+    bool wide_out = false;                  // and out's on 32-byte ones: whole sectors a store
+    bool early = false;                     // the addend is 16-bit and vec_add
 
     struct State {
         int64_t row;  // of out; -1: none
@@ -37,35 +56,74 @@ struct EpiOut {
     }
     __device__ __forceinline__ void end(State &, int64_t, int64_t) const {}
 
+    // the addend of 32 columns, fetched early where it is 16-bit and aligned
+    struct Ahead {
+        uint4 a[4];
+    };
+    __device__ __forceinline__ void fetch(const State &s, Ahead &h, int64_t col) const {
+        if (!early || s.row < 0 || col + 32 > n) return;
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(add) + s.row * ld_add + col);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h.a[i] = p[i];
+    }
+
+    template <class T>
+    __device__ __forceinline__ void add_fetched(float (&v)[32], const Ahead &h) const {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+            float2 f[4];
+            Pairs<T, 16>::unpack(h.a[j / 8], f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j + i] += i & 1 ? f[i / 2].y : f[i / 2].x;
+        }
+    }
     template <class T>
     __device__ __forceinline__ void load_add(float (&v)[32], int64_t row, int64_t col, int cols) const {
         const T *p = static_cast<const T *>(add) + row * ld_add + col;
         constexpr int N = 16 / (int)sizeof(T);
         if (vec_add && cols == 32) {
+            uint4 raw[32 / N];
+#pragma unroll
+            for (int j = 0; j < 32 / N; ++j) raw[j] = reinterpret_cast<const uint4 *>(p)[j];
 #pragma unroll
             for (int j = 0; j < 32; j += N) {
-                float f[N];
-                Vec<T, 16>::unpack(*reinterpret_cast<const uint4 *>(p + j), f);
+                float2 f[N / 2];
+                Pairs<T, 16>::unpack(raw[j / N], f);
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[j + i] += f[i];
+                for (int i = 0; i < N; ++i) v[j + i] += i & 1 ? f[i / 2].y : f[i / 2].x;
             }
         } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < cols) v[j] += Elem<T>::to(p[j]);
+            for (int j = 0; j < 32; ++j) {
+                const float a = j < cols ? Elem<T>::to(p[j]) : 0.0f;
+                at(v, j, a);
+            }
         }
+    }
+    // v[j] += a for a j that is not known at compile time (the ragged edge)
+    static __device__ __forceinline__ void at(float (&v)[32], int j, float a) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i == j) v[i] += a;
     }
     template <class T>
     __device__ __forceinline__ void store(const float (&v)[32], int64_t row, int64_t col, int cols) const {
         T *p = static_cast<T *>(out) + row * ld + col;
         constexpr int N = 16 / (int)sizeof(T);
         if (vec_out && cols == 32) {
+            uint4 raw[32 / N];
 #pragma unroll
             for (int j = 0; j < 32; j += N) {
-                float f[N];
+                float2 f[N / 2];
 #pragma unroll
-                for (int i = 0; i < N; ++i) f[i] = v[j + i];
-                *reinterpret_cast<uint4 *>(p + j) = Vec<T, 16>::pack(f);
+                for (int i = 0; i < N / 2; ++i) f[i] = make_float2(v[j + 2 * i], v[j + 2 * i + 1]);
+                raw[j / N] = Pairs<T, 16>::pack(f);
+            }
+            if (wide_out) {
+#pragma unroll
+                for (int j = 0; j < 32 / N; j += 2) store32(reinterpret_cast<uint4 *>(p) + j, raw[j], raw[j + 1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32 / N; ++j) reinterpret_cast<uint4 *>(p)[j] = raw[j];
             }
         } else {
 #pragma unroll
@@ -73,7 +131,8 @@ struct EpiOut {
                 if (j < cols) p[j] = Elem<T>::from(v[j]);
         }
     }
-    __device__ __forceinline__ void columns(State &s, float (&v)[32], int64_t, int64_t col) const {
+    __device__ __forceinline__ void columns(State &s, float (&v)[32], const float *tile_bias, const Ahead &h, int64_t,
+                                            int64_t col) const {
         if (s.row < 0) return;
         const int64_t row = s.row;
         const int cols = (int)(n - col < 32 ? n - col : 32);
@@ -81,13 +140,12 @@ struct EpiOut {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= s.f;
         }
-        if (bias) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < cols) v[j] += __ldg(bias + col + j);
-        }
+        if (bias) add_bias32(v, tile_bias);
         if (add) {
-            if (add_type == DNB_F32) load_add<float>(v, row, col, cols);
+            if (early && cols == 32) {
+                if (add_type == DNB_BF16) add_fetched<__nv_bfloat16>(v, h);
+                else add_fetched<__half>(v, h);
+            } else if (add_type == DNB_F32) load_add<float>(v, row, col, cols);
             else if (add_type == DNB_BF16) load_add<__nv_bfloat16>(v, row, col, cols);
             else load_add<__half>(v, row, col, cols);
         }
@@ -126,6 +184,7 @@ inline EpiOut epilogue(void *out, int64_t ld, int type, int64_t m, int64_t n) {
     e.m = m;
     e.n = n;
     e.vec_out = aligned16(out) && ld * dtype_size(type) % 16 == 0;
+    e.wide_out = reinterpret_cast<uintptr_t>(out) % 32 == 0 && ld * dtype_size(type) % 32 == 0;
     return e;
 }
 inline void add_to(EpiOut &e, const void *add, int64_t ld, int type) {
@@ -133,6 +192,7 @@ inline void add_to(EpiOut &e, const void *add, int64_t ld, int type) {
     e.ld_add = ld;
     e.add_type = type;
     e.vec_add = aligned16(add) && ld * dtype_size(type) % 16 == 0;
+    e.early = e.vec_add && type != DNB_F32;
 }
 
 // A pair's 256 x 256 tiles where they fill a B200's 74 pairs and there is more than one CTA's tile of rows;

@@ -67,8 +67,8 @@ struct GemmCfg {
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = STAGE >= 32768 ? 6 : STAGE >= 24576 ? 8 : 9;
     static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 256;
-    static_assert(BN % 32 == 0 && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 16 * STAGES + 64 + 8 * BN;
+    static_assert(BN % 64 == 0 && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
     static_assert(!B_MN || BROWS % 64 == 0, "an MN-major box is 64 wide");
 };
 
@@ -202,9 +202,8 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 columns of this warp's 32 lanes: v[j] is (lane, column j).
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-    uint32_t r[32];
+// 32 columns of this warp's 32 lanes: r[j] is (lane, column j), there after tmem_wait().
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
         "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
@@ -213,10 +212,18 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
 }
+// The registers pass through the wait, so that nothing that reads them moves above it.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])::"memory");
+}
+// The epilogue warps (4-7) meet.
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // The row tile and column tile of the t-th tile.
 __device__ __forceinline__ void tile_at(const GemmArgs &g, int m_tiles, int t, int &mt, int &nt) {
@@ -229,11 +236,17 @@ __device__ __forceinline__ void tile_at(const GemmArgs &g, int m_tiles, int t, i
 }  // namespace gemm
 
 // Epi: a struct passed by value to the kernel, with
+//   const float *bias;                                     a value per column, or NULL
 //   struct State;                                          a thread's row, kept over a tile's columns
+//   struct Ahead;                                          what 32 columns read from global memory
 //   void begin(State &, int64_t row, int64_t col0) const;
-//   void columns(State &, float (&v)[32], int64_t row, int64_t col) const;   32 columns from `col`
+//   void fetch(const State &, Ahead &, int64_t col) const; ahead of the accumulators
+//   void columns(State &, float (&v)[32], const float *bias, const Ahead &, int64_t row, int64_t col) const;
+//                                                          32 columns from `col`; bias: theirs, in shared memory
 //   void end(State &, int64_t row, int64_t col0) const;
-// All 32 lanes call each of them (rows beyond m included: the functions check).
+// All 32 lanes call each of them (rows beyond m included: the functions check). The bias of a tile and the
+// first columns' reads are on their way while the accumulators fill; read one by one when needed, 32 biases
+// cost 1.5 us a chunk of 32 columns, more than the product of a short k.
 template <class C, class Epi>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -344,29 +357,55 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     } else if (warp >= 4) {
         // epilogue: warp w reads tensor-memory lanes 32w..32w+31, a lane per row
         const int w = warp - 4;
+        float *bias = reinterpret_cast<float *>(tail + 16 * S + 64);  // [2][BN]
         int n = 0;
+        bool failed = false;
         for (int t = first; t < tiles; t += step, ++n) {
             const int b = n & 1;
             int mt, nt;
             tile_at(g, m_tiles, t, mt, nt);
-            const bool ok = mbar_wait(acc_full + 8 * b, (n >> 1) & 1, g, gave_up);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            fence_after();
             const int64_t row = (int64_t)mt * C::TM + (int64_t)rank * C::BM + w * 32 + lane, col0 = (int64_t)nt * C::BN;
-            const uint32_t at = tmem + ((uint32_t)(w * 32) << 16) + b * C::BN;
             typename Epi::State st;
             epi.begin(st, row, col0);
+            typename Epi::Ahead ahead[2];
+            epi.fetch(st, ahead[0], col0);
+            float *tile_bias = bias + b * C::BN;
+            if (epi.bias) {  // the buffer's last readers, two tiles ago, have met at the last tile's barrier
+                for (int c = threadIdx.x - 128; c < C::BN; c += 128)
+                    tile_bias[c] = col0 + c < g.n ? epi.bias[col0 + c] : 0.0f;
+                epilogue_sync();
+            }
+            // a warp that gave up goes on to the barriers, which the other warps may still wait at
+            if (!failed) failed = !__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b, (n >> 1) & 1, g, gave_up));
+            if (failed) continue;
+            fence_after();
+            const uint32_t at = tmem + ((uint32_t)(w * 32) << 16) + b * C::BN;
 #pragma unroll 1
-            for (int c = 0; c < C::BN; c += 32) {
+            for (int c = 0; c < C::BN; c += 64) {
                 if (col0 + c >= g.n) break;
-                float v[32];
+                uint32_t r[2][32];
                 if (k_blocks > 0) {
-                    tmem_load32(at + c, v);
+                    tmem_load32(at + c, r[0]);
+                    tmem_load32(at + c + 32, r[1]);
+                }
+                const bool second = col0 + c + 32 < g.n;
+                if (second) epi.fetch(st, ahead[1], col0 + c + 32);
+                if (k_blocks > 0) {
+                    tmem_wait(r[0]);
+                    tmem_wait(r[1]);
                 } else {  // a sum over nothing
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                    for (int j = 0; j < 32; ++j) r[0][j] = r[1][j] = 0u;
                 }
-                epi.columns(st, v, row, col0 + c);
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[0][j]);
+                epi.columns(st, v, tile_bias + c, ahead[0], row, col0 + c);
+                if (c + 64 < C::BN && col0 + c + 64 < g.n) epi.fetch(st, ahead[0], col0 + c + 64);
+                if (!second) break;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[1][j]);
+                epi.columns(st, v, tile_bias + c + 32, ahead[1], row, col0 + c + 32);
             }
             fence_before();
             __syncwarp();

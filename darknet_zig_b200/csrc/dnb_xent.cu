@@ -34,39 +34,47 @@ __global__ void __launch_bounds__(1024) k_kept_rows(const int32_t *labels, int64
     __shared__ int sums[32];
     __shared__ float tops[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int base = 0;
+    // a warp takes a run of 32-row blocks; a lane a row of each
+    const int64_t blocks = (batch + 31) / 32, run = (blocks + 31) / 32, b0 = warp * run,
+                  b1 = b0 + run < blocks ? b0 + run : blocks;
+    auto keeps = [&](int64_t b) {
+        const int64_t r = b * 32 + lane;
+        if (r >= batch) return false;
+        const int l = labels[r];
+        return l >= 0 && l < classes;
+    };
+    int mine = 0;
+#pragma unroll 8
+    for (int64_t b = b0; b < b1; ++b) mine += keeps(b);
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    int base = 0, all = 0;
+    for (int w = 0; w < 32; ++w) {
+        if (w < warp) base += sums[w];
+        all += sums[w];
+    }
+    if (threadIdx.x == 0) *count = all;
     float top = 0.0f;
-    for (int64_t r0 = 0; r0 < batch; r0 += 1024) {
-        const int64_t r = r0 + threadIdx.x;
-        const bool keep = r < batch && labels[r] >= 0 && labels[r] < classes;
+#pragma unroll 8
+    for (int64_t b = b0; b < b1; ++b) {
+        const bool keep = keeps(b);
         const unsigned mask = __ballot_sync(0xffffffffu, keep);
-        if (lane == 0) sums[warp] = __popc(mask);
-        __syncthreads();
-        if (warp == 0) {
-            int v = sums[lane];
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += u;
-            }
-            sums[lane] = v;
-        }
-        __syncthreads();
         if (keep) {
-            rows[base + (warp ? sums[warp - 1] : 0) + __popc(mask & ((1u << lane) - 1u))] = (int)r;
+            const int64_t r = b * 32 + lane;
+            rows[base + __popc(mask & ((1u << lane) - 1u))] = (int)r;
             if (factor) top = fmaxf(top, fabsf(factor[r]));
         }
-        base += sums[31];
-        __syncthreads();
+        base += __popc(mask);
     }
+    if (!factor) return;
     top = warp_max(top);
     if (lane == 0) tops[warp] = top;
-    if (threadIdx.x == 0) *count = base;
     __syncthreads();
-    if (factor && threadIdx.x == 0) {
+    if (threadIdx.x == 0) {
         for (int w = 1; w < 32; ++w) top = fmaxf(top, tops[w]);
-        int e = 0;
+        int e = 1;
         if (top > 0.0f && top <= 3.4e38f) frexpf(top, &e);
-        else e = 1;
         if (e > 120) e = 120;
         if (e < -120) e = -120;
         meta[0] = ldexpf(1.0f, 1 - e);
@@ -100,13 +108,13 @@ struct EpiStats {
     // nothing has been seen, and the sums come out as log sum exp's limits)
     static __device__ __forceinline__ float shift(float top) { return fabsf(top) < __int_as_float(0x7f800000) ? top : 0.0f; }
 
-    __device__ __forceinline__ void columns(State &s, float (&v)[32], int64_t row, int64_t col) const {
+    struct Ahead {};
+    __device__ __forceinline__ void fetch(const State &, Ahead &, int64_t) const {}
+
+    __device__ __forceinline__ void columns(State &s, float (&v)[32], const float *tile_bias, const Ahead &, int64_t row,
+                                            int64_t col) const {
         const int cols = (int)(n - col < 32 ? n - col : 32);
-        if (bias) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < cols) v[j] += __ldg(bias + col + j);
-        }
+        if (bias) add_bias32(v, tile_bias);
         if (cols < 32) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
@@ -133,41 +141,68 @@ struct EpiStats {
     }
 };
 
-// Merges the tiles of a row: 32 rows a block, 8 slices of the tiles each, added in a fixed order.
-__global__ void __launch_bounds__(256) k_xent_close(const float2 *part, const float *at_label, const int32_t *labels,
-                                                    const int *rows, const int *m_dev, int64_t m, int64_t tiles,
-                                                    int64_t classes, float *loss, float *lse) {
-    __shared__ float tops[8][32], sums[8][32];
+// Merges the tiles of a row: 32 rows a block, 32 slices of the tiles each; the maximum first, so that the sums
+// need no order, then the slices in a fixed one.
+__global__ void __launch_bounds__(1024) k_xent_close(const float2 *part, const float *at_label, const int32_t *labels,
+                                                     const int *rows, const int *m_dev, int64_t m, int64_t tiles,
+                                                     int64_t classes, float *loss, float *lse) {
+    __shared__ float red[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t row = (int64_t)blockIdx.x * 32 + tx, count = m_dev ? *m_dev : m;
-    float top = __int_as_float(0xff800000), sum = 0.0f;
-    if (row < count)
-#pragma unroll 4
-        for (int64_t t = ty; t < tiles; t += 8) {
-            const float2 p = part[t * m + row];
-            const float to = fmaxf(top, p.x);
-            sum = (sum == 0.0f ? 0.0f : sum * exp2f((top - to) * kLog2e)) + p.y * exp2f((p.x - to) * kLog2e);
-            top = to;
+    // a tile whose sum is 0 has only classes of -inf: its maximum stands for nothing
+    const float none = __int_as_float(0xff800000);
+    auto load = [&](int64_t t) {
+        float2 p = part[t * m + row];
+        if (p.y == 0.0f) p.x = none;
+        return p;
+    };
+    constexpr int kHeld = 8;
+    float2 held[kHeld];  // a slice's first tiles, read once
+    float top = none;
+    if (row < count) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int64_t t = ty + 32 * i;
+            held[i] = t < tiles ? load(t) : make_float2(none, 0.0f);
+            top = fmaxf(top, held[i].x);
         }
-    tops[ty][tx] = top;
-    sums[ty][tx] = sum;
+        for (int64_t t = ty + 32 * kHeld; t < tiles; t += 32) top = fmaxf(top, load(t).x);
+    }
+    red[ty][tx] = top;
     __syncthreads();
-    if (ty == 0 && row < count) {
-        for (int i = 1; i < 8; ++i) {
-            if (tops[i][tx] == __int_as_float(0xff800000)) continue;  // a slice of no tiles
-            const float to = fmaxf(top, tops[i][tx]);
-            sum = sum * exp2f((top - to) * kLog2e) + sums[i][tx] * exp2f((tops[i][tx] - to) * kLog2e);
-            top = to;
+    top = warp_max(red[tx][ty]);  // warp w: row w's slices
+    __syncthreads();
+    if (tx == 0) red[0][ty] = top;
+    __syncthreads();
+    top = red[0][tx];
+    __syncthreads();
+    float sum = 0.0f;
+    if (row < count) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (held[i].y != 0.0f) sum += held[i].y * exp2f((held[i].x - top) * kLog2e);
+        for (int64_t t = ty + 32 * kHeld; t < tiles; t += 32) {
+            const float2 p = load(t);
+            if (p.y != 0.0f) sum += p.y * exp2f((p.x - top) * kLog2e);
         }
+    }
+    red[ty][tx] = sum;
+    __syncthreads();
+    sum = warp_sum(red[tx][ty]);
+    __syncthreads();
+    if (tx == 0) red[0][ty] = sum;
+    __syncthreads();
+    if (ty != 0) return;
+    if (row < count) {
         const int64_t at = rows ? rows[row] : row;
         if (rows || (labels[at] >= 0 && labels[at] < classes)) {
-            const float l = top + logf(sum);
+            const float l = top + logf(red[0][tx]);
             lse[at] = l;
             loss[at] = l - at_label[row];
         }
     }
     // padding rows, each by the thread of its own index
-    if (ty == 0 && row < m && (labels[row] < 0 || labels[row] >= classes)) lse[row] = loss[row] = 0.0f;
+    if (row < m && (labels[row] < 0 || labels[row] >= classes)) lse[row] = loss[row] = 0.0f;
 }
 
 // ---- backward ----
@@ -221,14 +256,13 @@ struct EpiDelta {
                 if (j < cols) p[j] = Elem<T>::from(v[j] * kDeltaScale);
         }
     }
-    __device__ __forceinline__ void columns(State &s, float (&v)[32], int64_t row, int64_t col) const {
+    struct Ahead {};
+    __device__ __forceinline__ void fetch(const State &, Ahead &, int64_t) const {}
+    __device__ __forceinline__ void columns(State &s, float (&v)[32], const float *tile_bias, const Ahead &, int64_t row,
+                                            int64_t col) const {
         const int cols = (int)(n - col < 32 ? n - col : 32);
         if (s.kept) {
-            if (bias) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (j < cols) v[j] += __ldg(bias + col + j);
-            }
+            if (bias) add_bias32(v, tile_bias);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = -exp2f((v[j] - s.lse) * kLog2e);
             const int64_t at = (int64_t)s.at - col;
@@ -407,7 +441,7 @@ dnb_status dnb_connected_xent_forward(const void *x, int64_t ldx, const void *w,
             ? launch_gemm<GemmCfg<2, 256, false, false>>(a, b, dtype, batch, classes, inputs, e, ds, s, what, f.count)
             : launch_gemm<GemmCfg<1, 128, false, false>>(a, b, dtype, batch, classes, inputs, e, ds, s, what, f.count);
     DNB_TRY(st);
-    k_xent_close<<<(unsigned)((batch + 31) / 32), 256, 0, s>>>(f.part, f.at_label, labels, f.rows, f.count, batch,
+    k_xent_close<<<(unsigned)((batch + 31) / 32), 1024, 0, s>>>(f.part, f.at_label, labels, f.rows, f.count, batch,
                                                                f.tiles, classes, loss, lse);
     return after_launch(s, what);
 }

@@ -125,6 +125,15 @@ def test_forward_infinities(cuda):
     assert torch.isnan(loss[4]) and torch.isnan(lse[4]) and torch.isfinite(loss[5:]).all()
 
 
+def test_forward_impossible_tile_beside_small_outputs(cuda):
+    """A whole tile of classes that cannot occur, and the others far below 0."""
+    x, w, b, labels = _make(16, 20, 64, 700, torch.bfloat16)
+    labels[:] = 600
+    b[:300] = float("-inf")
+    b[300:] -= 300.0
+    _check_forward(x, w, b, labels)
+
+
 def _backward(x, w, b, labels, lse, rs, scale, dw_type=None, accumulate=0, want=(1, 1, 1), pad=0, workspace=None):
     from darknet_zig_b200 import gpu
 
