@@ -11,15 +11,18 @@ __device__ __forceinline__ void store32(uint4 *p, uint4 a, uint4 b) {
                  : "memory");
 }
 // A tile's biases from shared memory (the same address in every lane).
-__device__ __forceinline__ void add_bias32(float (&v)[32], const float *bias) {
+__device__ __forceinline__ void add_bias32(float2 (&v)[16], const float *bias) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-        const float4 b = *reinterpret_cast<const float4 *>(bias + j);
-        v[j] += b.x;
-        v[j + 1] += b.y;
-        v[j + 2] += b.z;
-        v[j + 3] += b.w;
+    for (int j = 0; j < 16; j += 2) {
+        const float4 b = *reinterpret_cast<const float4 *>(bias + 2 * j);
+        v[j] = __fadd2_rn(v[j], make_float2(b.x, b.y));
+        v[j + 1] = __fadd2_rn(v[j + 1], make_float2(b.z, b.w));
     }
+}
+template <int A>
+__device__ __forceinline__ void act32(float2 (&v)[16], int a) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = act_pair<A>(v[j], a);
 }
 
 // out = act(f * acc + bias[n] + add[m][n]) (add may be out), f = alpha * *alpha_dev * row_factor[row].
@@ -68,17 +71,17 @@ struct EpiOut {
     }
 
     template <class T>
-    __device__ __forceinline__ void add_fetched(float (&v)[32], const Ahead &h) const {
+    __device__ __forceinline__ void add_fetched(float2 (&v)[16], const Ahead &h) const {
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
+        for (int j = 0; j < 4; ++j) {
             float2 f[4];
-            Pairs<T, 16>::unpack(h.a[j / 8], f);
+            Pairs<T, 16>::unpack(h.a[j], f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[j + i] += i & 1 ? f[i / 2].y : f[i / 2].x;
+            for (int i = 0; i < 4; ++i) v[4 * j + i] = __fadd2_rn(v[4 * j + i], f[i]);
         }
     }
     template <class T>
-    __device__ __forceinline__ void load_add(float (&v)[32], int64_t row, int64_t col, int cols) const {
+    __device__ __forceinline__ void load_add(float2 (&v)[16], int64_t row, int64_t col, int cols) const {
         const T *p = static_cast<const T *>(add) + row * ld_add + col;
         constexpr int N = 16 / (int)sizeof(T);
         if (vec_add && cols == 32) {
@@ -86,37 +89,32 @@ struct EpiOut {
 #pragma unroll
             for (int j = 0; j < 32 / N; ++j) raw[j] = reinterpret_cast<const uint4 *>(p)[j];
 #pragma unroll
-            for (int j = 0; j < 32; j += N) {
+            for (int j = 0; j < 32 / N; ++j) {
                 float2 f[N / 2];
-                Pairs<T, 16>::unpack(raw[j / N], f);
+                Pairs<T, 16>::unpack(raw[j], f);
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[j + i] += i & 1 ? f[i / 2].y : f[i / 2].x;
+                for (int i = 0; i < N / 2; ++i) v[j * N / 2 + i] = __fadd2_rn(v[j * N / 2 + i], f[i]);
             }
         } else {
-            for (int j = 0; j < 32; ++j) {
-                const float a = j < cols ? Elem<T>::to(p[j]) : 0.0f;
-                at(v, j, a);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                if (2 * j < cols) v[j].x += Elem<T>::to(p[2 * j]);
+                if (2 * j + 1 < cols) v[j].y += Elem<T>::to(p[2 * j + 1]);
             }
         }
     }
-    // v[j] += a for a j that is not known at compile time (the ragged edge)
-    static __device__ __forceinline__ void at(float (&v)[32], int j, float a) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i == j) v[i] += a;
-    }
     template <class T>
-    __device__ __forceinline__ void store(const float (&v)[32], int64_t row, int64_t col, int cols) const {
+    __device__ __forceinline__ void store(const float2 (&v)[16], int64_t row, int64_t col, int cols) const {
         T *p = static_cast<T *>(out) + row * ld + col;
         constexpr int N = 16 / (int)sizeof(T);
         if (vec_out && cols == 32) {
             uint4 raw[32 / N];
 #pragma unroll
-            for (int j = 0; j < 32; j += N) {
+            for (int j = 0; j < 32 / N; ++j) {
                 float2 f[N / 2];
 #pragma unroll
-                for (int i = 0; i < N / 2; ++i) f[i] = make_float2(v[j + 2 * i], v[j + 2 * i + 1]);
-                raw[j / N] = Pairs<T, 16>::pack(f);
+                for (int i = 0; i < N / 2; ++i) f[i] = v[j * N / 2 + i];
+                raw[j] = Pairs<T, 16>::pack(f);
             }
             if (wide_out) {
 #pragma unroll
@@ -127,18 +125,20 @@ struct EpiOut {
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < cols) p[j] = Elem<T>::from(v[j]);
+            for (int j = 0; j < 16; ++j) {
+                if (2 * j < cols) p[2 * j] = Elem<T>::from(v[j].x);
+                if (2 * j + 1 < cols) p[2 * j + 1] = Elem<T>::from(v[j].y);
+            }
         }
     }
-    __device__ __forceinline__ void columns(State &s, float (&v)[32], const float *tile_bias, const Ahead &h, int64_t,
+    __device__ __forceinline__ void columns(State &s, float2 (&v)[16], const float *tile_bias, const Ahead &h, int64_t,
                                             int64_t col) const {
         if (s.row < 0) return;
         const int64_t row = s.row;
         const int cols = (int)(n - col < 32 ? n - col : 32);
         if (s.f != 1.0f) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= s.f;
+            for (int j = 0; j < 16; ++j) v[j] = __fmul2_rn(v[j], both(s.f));
         }
         if (bias) add_bias32(v, tile_bias);
         if (add) {
@@ -151,18 +151,9 @@ struct EpiOut {
         }
         switch (act) {
         case DNB_ACT_LINEAR: break;
-        case DNB_ACT_LEAKY:
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = act_fwd<DNB_ACT_LEAKY>(v[j], act);
-            break;
-        case DNB_ACT_RELU:
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = act_fwd<DNB_ACT_RELU>(v[j], act);
-            break;
-        case DNB_ACT_LOGISTIC:
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = act_fwd<DNB_ACT_LOGISTIC>(v[j], act);
-            break;
+        case DNB_ACT_LEAKY: act32<DNB_ACT_LEAKY>(v, act); break;
+        case DNB_ACT_RELU: act32<DNB_ACT_RELU>(v, act); break;
+        case DNB_ACT_LOGISTIC: act32<DNB_ACT_LOGISTIC>(v, act); break;
         default: activate_any(v, act);
         }
         if (out_type == DNB_F32) store<float>(v, row, col, cols);
@@ -170,9 +161,9 @@ struct EpiOut {
         else store<__half>(v, row, col, cols);
     }
     static __device__ __noinline__ float activate_one(float v, int a) { return act_fwd_any(v, a); }
-    static __device__ __forceinline__ void activate_any(float (&v)[32], int a) {
+    static __device__ __forceinline__ void activate_any(float2 (&v)[16], int a) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = activate_one(v[j], a);
+        for (int j = 0; j < 16; ++j) v[j] = make_float2(activate_one(v[j].x, a), activate_one(v[j].y, a));
     }
 };
 

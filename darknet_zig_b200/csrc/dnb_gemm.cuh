@@ -8,8 +8,9 @@
 //
 // A CTA (CTAS = 1) or a pair on neighbouring SMs (CTAS = 2, cta_group::2) owns one output tile of
 // 128*CTAS x BN at a time. Warp 0 issues the loads into a ring of stages (64 k each), warp 1 of the pair's
-// first CTA issues the products into one of two accumulators in tensor memory, warps 4-7 take the other
-// accumulator through the epilogue meanwhile. A pair halves the operand traffic per SM: each CTA holds its
+// first CTA issues the products into one of two accumulators in tensor memory, warps 4-11 take the other
+// accumulator through the epilogue meanwhile (two warps a scheduler, each half of the columns: one alone
+// leaves its latencies bare and took 7 us for a tile that two finish in 3). A pair halves the operand traffic per SM: each CTA holds its
 // own 128 rows of A and half of B's rows, and the products read both CTAs' shared memory.
 //
 // Every wait is bounded (dnb_set_wait_limit_ms): a role whose wait gives up sets the error word and
@@ -52,7 +53,8 @@ struct GemmArgs {
     unsigned *error_word;
 };
 
-constexpr int kGemmThreads = 256;
+constexpr int kGemmThreads = 384;  // 4 warps of roles, 8 of epilogue
+constexpr int kEpilogueWarps = 8;
 constexpr int kBlockK = 64;
 constexpr unsigned DEVERR_WAIT_GEMM = 8u;  // a role of a product gave up waiting
 
@@ -68,7 +70,7 @@ struct GemmCfg {
     static constexpr int STAGES = STAGE >= 32768 ? 6 : STAGE >= 24576 ? 8 : 9;
     static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
     static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 16 * STAGES + 64 + 8 * BN;
-    static_assert(BN % 64 == 0 && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
+    static_assert(BN % 128 == 0 && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
     static_assert(!B_MN || BROWS % 64 == 0, "an MN-major box is 64 wide");
 };
 
@@ -84,8 +86,10 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {  // bar: a shared::cluster address
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrives at a shared::cluster address for reads of tensor memory, which the wait for them and the tcgen05 fence
+// before it order: relaxed, for a release would wait for the epilogue's stores too (0.7 us a tile).
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -222,8 +226,8 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
                    "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
                    "+r"(r[30]), "+r"(r[31])::"memory");
 }
-// The epilogue warps (4-7) meet.
-__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The epilogue warps meet.
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // The row tile and column tile of the t-th tile.
 __device__ __forceinline__ void tile_at(const GemmArgs &g, int m_tiles, int t, int &mt, int &nt) {
@@ -241,8 +245,10 @@ __device__ __forceinline__ void tile_at(const GemmArgs &g, int m_tiles, int t, i
 //   struct Ahead;                                          what 32 columns read from global memory
 //   void begin(State &, int64_t row, int64_t col0) const;
 //   void fetch(const State &, Ahead &, int64_t col) const; ahead of the accumulators
-//   void columns(State &, float (&v)[32], const float *bias, const Ahead &, int64_t row, int64_t col) const;
+//   void columns(State &, float2 (&v)[16], const float *bias, const Ahead &, int64_t row, int64_t col) const;
 //                                                          32 columns from `col`; bias: theirs, in shared memory
+//                                                          (row's columns are seen in two halves of the tile, by
+//                                                          two threads)
 //   void end(State &, int64_t row, int64_t col0) const;
 // All 32 lanes call each of them (rows beyond m included: the functions check). The bias of a tile and the
 // first columns' reads are on their way while the accumulators fill; read one by one when needed, 32 biases
@@ -272,7 +278,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + 8 * b, 1);
-            mbar_init(acc_empty + 8 * b, 4 * CTAS);
+            mbar_init(acc_empty + 8 * b, kEpilogueWarps * CTAS);
         }
         *gave_up = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -355,8 +361,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             if (ok) commit<CTAS>(acc_full + 8 * b);
         }
     } else if (warp >= 4) {
-        // epilogue: warp w reads tensor-memory lanes 32w..32w+31, a lane per row
-        const int w = warp - 4;
+        // epilogue: a warp reads its quarter of the tensor memory's lanes (a lane a row) and half of the columns
+        constexpr int EW = C::BN / 2;
+        const int w = warp & 3, half = (warp - 4) >> 2;
         float *bias = reinterpret_cast<float *>(tail + 16 * S + 64);  // [2][BN]
         int n = 0;
         bool failed = false;
@@ -364,53 +371,51 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const int b = n & 1;
             int mt, nt;
             tile_at(g, m_tiles, t, mt, nt);
-            const int64_t row = (int64_t)mt * C::TM + (int64_t)rank * C::BM + w * 32 + lane, col0 = (int64_t)nt * C::BN;
+            const int64_t row = (int64_t)mt * C::TM + (int64_t)rank * C::BM + w * 32 + lane,
+                          tile0 = (int64_t)nt * C::BN, col0 = tile0 + half * EW;
             typename Epi::State st;
             epi.begin(st, row, col0);
             typename Epi::Ahead ahead[2];
             epi.fetch(st, ahead[0], col0);
-            float *tile_bias = bias + b * C::BN;
             if (epi.bias) {  // the buffer's last readers, two tiles ago, have met at the last tile's barrier
-                for (int c = threadIdx.x - 128; c < C::BN; c += 128)
-                    tile_bias[c] = col0 + c < g.n ? epi.bias[col0 + c] : 0.0f;
+                const int c = threadIdx.x - 128;
+                if (c < C::BN) bias[b * C::BN + c] = tile0 + c < g.n ? epi.bias[tile0 + c] : 0.0f;
                 epilogue_sync();
             }
+            const float *tile_bias = bias + b * C::BN + half * EW;
             // a warp that gave up goes on to the barriers, which the other warps may still wait at
             if (!failed) failed = !__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b, (n >> 1) & 1, g, gave_up));
             if (failed) continue;
             fence_after();
-            const uint32_t at = tmem + ((uint32_t)(w * 32) << 16) + b * C::BN;
+            const uint32_t at = tmem + ((uint32_t)(w * 32) << 16) + b * C::BN + half * EW;
 #pragma unroll 1
-            for (int c = 0; c < C::BN; c += 64) {
-                if (col0 + c >= g.n) break;
-                uint32_t r[2][32];
-                if (k_blocks > 0) {
-                    tmem_load32(at + c, r[0]);
-                    tmem_load32(at + c + 32, r[1]);
+            for (int c = 0; c < EW; c += 64) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t col = col0 + c + 32 * h;
+                    uint32_t r[32];
+                    __syncwarp();  // the loads are the whole warp's
+                    if (k_blocks > 0) tmem_load32(at + c + 32 * h, r);
+                    if (c + 32 * (h + 1) < EW && col + 32 < g.n) epi.fetch(st, ahead[h ^ 1], col + 32);
+                    if (k_blocks > 0) {
+                        tmem_wait(r);
+                    } else {  // a sum over nothing
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[j] = 0u;
+                    }
+                    if (h == 1 && c + 64 >= EW) {  // all read: the next products may overwrite the accumulators
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0)
+                            mbar_arrive_relaxed(CTAS == 2 ? map_rank(acc_empty + 8 * b, 0) : acc_empty + 8 * b);
+                    }
+                    float2 v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                    if (col < g.n) epi.columns(st, v, tile_bias + c + 32 * h, ahead[h], row, col);
                 }
-                const bool second = col0 + c + 32 < g.n;
-                if (second) epi.fetch(st, ahead[1], col0 + c + 32);
-                if (k_blocks > 0) {
-                    tmem_wait(r[0]);
-                    tmem_wait(r[1]);
-                } else {  // a sum over nothing
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) r[0][j] = r[1][j] = 0u;
-                }
-                float v[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[0][j]);
-                epi.columns(st, v, tile_bias + c, ahead[0], row, col0 + c);
-                if (c + 64 < C::BN && col0 + c + 64 < g.n) epi.fetch(st, ahead[0], col0 + c + 64);
-                if (!second) break;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[1][j]);
-                epi.columns(st, v, tile_bias + c + 32, ahead[1], row, col0 + c + 32);
             }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(CTAS == 2 ? map_rank(acc_empty + 8 * b, 0) : acc_empty + 8 * b);
-            epi.end(st, row, col0);
+            if (col0 < g.n) epi.end(st, row, col0);
         }
     }
     __syncwarp();

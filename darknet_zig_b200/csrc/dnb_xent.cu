@@ -92,7 +92,7 @@ struct EpiStats {
     float2 *part;             // [tile][m]
     float *at_label;          // [m]
     int64_t m, n;
-    int bn;
+    int bn;  // columns of a thread's part: half a tile
 
     struct State {
         float top, sum;
@@ -111,30 +111,38 @@ struct EpiStats {
     struct Ahead {};
     __device__ __forceinline__ void fetch(const State &, Ahead &, int64_t) const {}
 
-    __device__ __forceinline__ void columns(State &s, float (&v)[32], const float *tile_bias, const Ahead &, int64_t row,
-                                            int64_t col) const {
+    __device__ __forceinline__ void columns(State &s, float2 (&v)[16], const float *tile_bias, const Ahead &,
+                                            int64_t row, int64_t col) const {
         const int cols = (int)(n - col < 32 ? n - col : 32);
+        const float none = __int_as_float(0xff800000);
         if (bias) add_bias32(v, tile_bias);
         if (cols < 32) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j >= cols) v[j] = __int_as_float(0xff800000);
+            for (int j = 0; j < 16; ++j) {
+                if (2 * j >= cols) v[j].x = none;
+                if (2 * j + 1 >= cols) v[j].y = none;
+            }
         }
         const int64_t at = (int64_t)s.label - col;
         if (at >= 0 && at < cols) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j == at) at_label[row] = v[j];
+            for (int j = 0; j < 16; ++j) {
+                if (2 * j == at) at_label[row] = v[j].x;
+                if (2 * j + 1 == at) at_label[row] = v[j].y;
+            }
         }
         float top = s.top;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, fmaxf(v[j].x, v[j].y));
         const float to = shift(top);
-        float sum = s.sum == 0.0f ? 0.0f : s.sum * exp2f((shift(s.top) - to) * kLog2e);
+        float2 sum = make_float2(s.sum == 0.0f ? 0.0f : s.sum * quick_exp(shift(s.top) - to), 0.0f);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) sum += exp2f((v[j] - to) * kLog2e);
+        for (int j = 0; j < 16; ++j) {
+            const float2 d = __fadd2_rn(v[j], both(-to));
+            sum = __fadd2_rn(sum, make_float2(quick_exp(d.x), quick_exp(d.y)));
+        }
         s.top = top;
-        s.sum = sum;
+        s.sum = sum.x + sum.y;
     }
     __device__ __forceinline__ void end(State &s, int64_t row, int64_t col0) const {
         if (row < (m_dev ? *m_dev : m)) part[(col0 / bn) * m + row] = make_float2(shift(s.top), s.sum);
@@ -240,40 +248,47 @@ struct EpiDelta {
     __device__ __forceinline__ void end(State &, int64_t, int64_t) const {}
 
     template <class T>
-    __device__ __forceinline__ void store(const float (&v)[32], int64_t row, int64_t col, int cols) const {
+    __device__ __forceinline__ void store(const float2 (&v)[16], int64_t row, int64_t col, int cols) const {
         T *p = static_cast<T *>(d) + row * ld + col;
         if (cols == 32) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-                float f[8];
+            for (int j = 0; j < 4; ++j) {
+                float2 f[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = v[j + i] * kDeltaScale;
-                *reinterpret_cast<uint4 *>(p + j) = Vec<T, 16>::pack(f);
+                for (int i = 0; i < 4; ++i) f[i] = __fmul2_rn(v[4 * j + i], both(kDeltaScale));
+                reinterpret_cast<uint4 *>(p)[j] = Pairs<T, 16>::pack(f);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < cols) p[j] = Elem<T>::from(v[j] * kDeltaScale);
+            for (int j = 0; j < 16; ++j) {
+                if (2 * j < cols) p[2 * j] = Elem<T>::from(v[j].x * kDeltaScale);
+                if (2 * j + 1 < cols) p[2 * j + 1] = Elem<T>::from(v[j].y * kDeltaScale);
+            }
         }
     }
     struct Ahead {};
     __device__ __forceinline__ void fetch(const State &, Ahead &, int64_t) const {}
-    __device__ __forceinline__ void columns(State &s, float (&v)[32], const float *tile_bias, const Ahead &, int64_t row,
-                                            int64_t col) const {
+    __device__ __forceinline__ void columns(State &s, float2 (&v)[16], const float *tile_bias, const Ahead &,
+                                            int64_t row, int64_t col) const {
         const int cols = (int)(n - col < 32 ? n - col : 32);
         if (s.kept) {
             if (bias) add_bias32(v, tile_bias);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = -exp2f((v[j] - s.lse) * kLog2e);
+            for (int j = 0; j < 16; ++j) {
+                const float2 z = __fadd2_rn(v[j], both(-s.lse));
+                v[j] = make_float2(-quick_exp(z.x), -quick_exp(z.y));
+            }
             const int64_t at = (int64_t)s.at - col;
             if (at >= 0 && at < 32) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (j == at) v[j] += 1.0f;
+                for (int j = 0; j < 16; ++j) {
+                    if (2 * j == at) v[j].x += 1.0f;
+                    if (2 * j + 1 == at) v[j].y += 1.0f;
+                }
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+            for (int j = 0; j < 16; ++j) v[j] = both(0.0f);
         }
         if (s.kept || s.zero) {
             if (dtype == DNB_BF16) store<__nv_bfloat16>(v, row, col, cols);
@@ -281,19 +296,23 @@ struct EpiDelta {
         }
         if (sums) {  // lane j ends up with column j's sum over the warp's 32 rows
             const int lane = threadIdx.x & 31;
+            float u[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= s.f;
+            for (int j = 0; j < 16; ++j) {
+                u[2 * j] = v[j].x * s.f;
+                u[2 * j + 1] = v[j].y * s.f;
+            }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 const bool up = lane & o;
 #pragma unroll
                 for (int j = 0; j < o; ++j) {
-                    const float send = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
-                    v[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                    const float send = up ? u[j] : u[j + o], keep = up ? u[j + o] : u[j];
+                    u[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
                 }
             }
             const int64_t block = row / 32;
-            if (block * 32 < *count && lane < cols) sums[block * ld + col + lane] = v[0];
+            if (block * 32 < *count && lane < cols) sums[block * ld + col + lane] = u[0];
         }
     }
 };
@@ -333,7 +352,7 @@ struct FwdSpace {
 FwdSpace fwd_space(void *ws, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t m, int64_t k, int64_t n) {
     Carver c(ws);
     FwdSpace f{};
-    f.bn = big_tiles(m, n) ? 256 : 128;
+    f.bn = (big_tiles(m, n) ? 256 : 128) / 2;  // the epilogue's half tiles
     f.tiles = (n + f.bn - 1) / f.bn;
     f.part = static_cast<float2 *>(c.take(f.tiles * m * 8));
     f.at_label = static_cast<float *>(c.take(m * 4));
@@ -437,7 +456,7 @@ dnb_status dnb_connected_xent_forward(const void *x, int64_t ldx, const void *w,
     if (f.w) b = {f.w, packed_ld(inputs)};
     EpiStats e{biases, labels, f.rows, f.count, f.part, f.at_label, batch, classes, f.bn};
     const dnb_status st =
-        f.bn == 256
+        f.bn == 128
             ? launch_gemm<GemmCfg<2, 256, false, false>>(a, b, dtype, batch, classes, inputs, e, ds, s, what, f.count)
             : launch_gemm<GemmCfg<1, 128, false, false>>(a, b, dtype, batch, classes, inputs, e, ds, s, what, f.count);
     DNB_TRY(st);
