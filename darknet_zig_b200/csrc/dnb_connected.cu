@@ -23,45 +23,56 @@ struct RowsArgs {
     int act, out_type;
 };
 
-// MB rows of x at a time; a block of 8 warps, WPR of them share an output and split its k.
+// MB rows of x at a time; a block of 8 warps, WPR of them share an output and split its k. A lane has U vectors of
+// w (and as many of x, which the L1 cache holds) on their way before it needs the first.
 template <class T, int VB, int MB>
 __global__ void __launch_bounds__(256) k_rows(const __grid_constant__ RowsArgs a, int wpr) {
-    using V = Vec<T, VB>;
+    using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
-    constexpr int N = V::N;
+    constexpr int N = V::N, P = V::P, U = MB == 1 ? 8 : 4;
     __shared__ float red[8][MB];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, outs = 8 / wpr;
     const int64_t row = (int64_t)blockIdx.x * outs + warp / wpr;
     const int part = warp % wpr;
     const int64_t m0 = (int64_t)blockIdx.y * MB;
-    const T *x = static_cast<const T *>(a.x), *w = static_cast<const T *>(a.w) + row * a.ldw;
-    float acc[MB] = {};
+    const T *x = static_cast<const T *>(a.x) + m0 * a.ldx, *w = static_cast<const T *>(a.w) + row * a.ldw;
+    const int rows = (int)(a.m - m0 < MB ? a.m - m0 : MB);
+    float2 acc[MB] = {};
     if (row < a.n) {
         const int64_t vecs = a.k / N;
-#pragma unroll 4
-        for (int64_t i = part * 32 + lane; i < vecs; i += wpr * 32) {
-            float fw[N];
-            V::unpack(__ldg(reinterpret_cast<const Raw *>(w + i * N)), fw);
+        const int step = wpr * 32;
+        int64_t i = part * 32 + lane;
+        auto take = [&](Raw rw, int64_t at) {
+            float2 fw[P];
+            V::unpack(rw, fw);
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
-                if (m0 + b >= a.m) break;
-                float fx[N];
-                V::unpack(__ldg(reinterpret_cast<const Raw *>(x + (m0 + b) * a.ldx + i * N)), fx);
+                if (b >= rows) break;
+                float2 fx[P];
+                V::unpack(__ldg(reinterpret_cast<const Raw *>(x + b * a.ldx + at * N)), fx);
 #pragma unroll
-                for (int j = 0; j < N; ++j) acc[b] = __fmaf_rn(fx[j], fw[j], acc[b]);
+                for (int j = 0; j < P; ++j) acc[b] = __ffma2_rn(fx[j], fw[j], acc[b]);
             }
+        };
+        for (; i + (U - 1) * step < vecs; i += U * step) {
+            Raw rw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) rw[u] = __ldcs(reinterpret_cast<const Raw *>(w + (i + u * step) * N));
+#pragma unroll
+            for (int u = 0; u < U; ++u) take(rw[u], i + u * step);
         }
+        for (; i < vecs; i += step) take(__ldcs(reinterpret_cast<const Raw *>(w + i * N)), i);
         // the last k % N elements
-        const int64_t i = vecs * N + lane;
-        if (part == 0 && i < a.k)
+        const int64_t last = vecs * N + lane;
+        if (part == 0 && last < a.k)
 #pragma unroll
             for (int b = 0; b < MB; ++b)
-                if (m0 + b < a.m) acc[b] = __fmaf_rn(Elem<T>::to(x[(m0 + b) * a.ldx + i]), Elem<T>::to(w[i]), acc[b]);
+                if (b < rows) acc[b].x = __fmaf_rn(Elem<T>::to(x[b * a.ldx + last]), Elem<T>::to(w[last]), acc[b].x);
     }
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
-        acc[b] = warp_sum(acc[b]);
-        if (lane == 0) red[warp][b] = acc[b];
+        const float s = warp_sum(acc[b].x + acc[b].y);
+        if (lane == 0) red[warp][b] = s;
     }
     __syncthreads();
     // a thread per (output, row): the parts added in order
@@ -84,8 +95,7 @@ dnb_status run_rows(const RowsArgs &a, cudaStream_t s, const char *what) {
     const int64_t outs = 8 / wpr, blocks = (a.n + outs - 1) / outs;
     if (blocks > 0x7fffffffll) return fail(DNB_ERR_UNSUPPORTED, "%s: too many outputs", what);
     if (a.m == 1) k_rows<T, VB, 1><<<dim3((unsigned)blocks, 1), 256, 0, s>>>(a, wpr);
-    else if (a.m == 2) k_rows<T, VB, 2><<<dim3((unsigned)blocks, 1), 256, 0, s>>>(a, wpr);
-    else k_rows<T, VB, 4><<<dim3((unsigned)blocks, (unsigned)((a.m + 3) / 4)), 256, 0, s>>>(a, wpr);
+    else k_rows<T, VB, 2><<<dim3((unsigned)blocks, (unsigned)((a.m + 1) / 2)), 256, 0, s>>>(a, wpr);
     return after_launch(s, what);
 }
 
@@ -131,7 +141,7 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
 
 constexpr int kDzRows = 64;
 
-constexpr int64_t kFewRows = 4;
+constexpr int64_t kFewRows = 2;  // [1 | 2 | 4 rows, 4096] x [4096, 4096]^T
 
 struct FwdSpace {
     void *x, *w;
@@ -209,7 +219,7 @@ dnb_status dnb_connected_act_forward(const void *x, int64_t ldx, const void *w, 
         RowsArgs a{x, w, residual, y, biases, ldx, ldw, ldr, ldy, batch, outputs, inputs, act, dtype};
         a.n = outputs;
         a.k = inputs;
-        if (batch > 4 * 65535) return fail(DNB_ERR_UNSUPPORTED, "%s: too many rows without inputs", what);
+        if (batch > 2 * 65535) return fail(DNB_ERR_UNSUPPORTED, "%s: too many rows without inputs", what);
         const uintptr_t al = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) |
                              (batch > 1 ? (uintptr_t)ldx * 2 : 0) | (outputs > 1 ? (uintptr_t)ldw * 2 : 0);
         return dispatch_dtype16(dtype, [&]<class T>() {
@@ -226,7 +236,7 @@ dnb_status dnb_connected_act_forward(const void *x, int64_t ldx, const void *w, 
     e.bias = biases;
     e.act = act;
     if (residual) add_to(e, residual, ldr, dtype);
-    return product<false, false>(a, b, dtype, batch, outputs, inputs, e, ds, s, what);
+    return product(false, false, a, b, dtype, batch, outputs, inputs, e, ds, s, what);
 }
 
 dnb_status dnb_connected_act_backward_workspace(const void *x, int64_t ldx, const void *w, int64_t ldw,
@@ -348,7 +358,7 @@ dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w,
         if (f.w) b = {f.w, packed_ld(inputs)};
         EpiOut e = epilogue(dx, lddx, dtype, batch, inputs);
         if (add_x) add_to(e, dx, lddx, dtype);
-        const dnb_status st = product<false, true>(d, b, dtype, batch, inputs, outputs, e, ds, s, what);
+        const dnb_status st = product(false, true, d, b, dtype, batch, inputs, outputs, e, ds, s, what);
         DNB_TRY(st);
     }
     if (weight_updates) {
@@ -356,7 +366,7 @@ dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w,
         if (f.x) b = {f.x, packed_ld(inputs)};
         EpiOut e = epilogue(weight_updates, lddw, updates_dtype, outputs, inputs);
         if (add_w) add_to(e, weight_updates, lddw, updates_dtype);
-        const dnb_status st = product<true, true>(d, b, dtype, outputs, inputs, batch, e, ds, s, what);
+        const dnb_status st = product(true, true, d, b, dtype, outputs, inputs, batch, e, ds, s, what);
         DNB_TRY(st);
     }
     return DNB_OK;

@@ -186,17 +186,10 @@ inline void add_to(EpiOut &e, const void *add, int64_t ld, int type) {
     e.early = e.vec_add && type != DNB_F32;
 }
 
-// A pair's 256 x 256 tiles where they fill a B200's 74 pairs and there is more than one CTA's tile of rows;
-// else single CTAs' 128 x 128 tiles. (Workspaces depend on it: a constant, not the current device's count.)
-inline bool big_tiles(int64_t m, int64_t n) { return m > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= 74; }
-
-template <bool A_MN, bool B_MN>
-dnb_status product(const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k, const EpiOut &e,
-                   const DeviceState *ds, cudaStream_t s, const char *what, const int *m_dev = nullptr,
-                   const int *k_dev = nullptr) {
-    if (big_tiles(m, n))
-        return launch_gemm<GemmCfg<2, 256, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
-    return launch_gemm<GemmCfg<1, 128, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
-}
+// The product with this epilogue, in the tiles that pick_tiles names; a_mn / b_mn: MN-major operands. With
+// m_dev / k_dev, m and k are what they may reach. dnb_product.cu.
+dnb_status product(bool a_mn, bool b_mn, const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k,
+                   const EpiOut &e, const DeviceState *ds, cudaStream_t s, const char *what,
+                   const int *m_dev = nullptr, const int *k_dev = nullptr);
 
 }  // namespace dnb

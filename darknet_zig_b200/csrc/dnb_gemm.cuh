@@ -48,6 +48,7 @@ struct GemmArgs {
     int m_tiles, n_tiles, k_blocks;
     int band;       // output tiles are taken in bands of this many row tiles, down the rows first
     unsigned idesc; // the tensor core's instruction descriptor
+    unsigned stage_bytes;  // what a CTA's loads of a stage bring
     const int *m_dev, *k_dev;  // the rows / the reduction's length where the device knows them (NULL: as above)
     unsigned long long wait_ns;
     unsigned *error_word;
@@ -67,10 +68,12 @@ struct GemmCfg {
     static constexpr int BROWS = BN / CTAS;    // B rows one CTA holds
     static constexpr int A_BYTES = BM * kBlockK * 2, B_BYTES = BROWS * kBlockK * 2;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = STAGE >= 32768 ? 6 : STAGE >= 24576 ? 8 : 9;
-    static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr int STAGES = STAGE >= 32768 ? 6 : STAGE >= 24576 ? 8 : 10;
+    static constexpr int TMEM_COLS = 2 * BN;
+    static constexpr int PARTS = BN >= 128 ? 2 : 1;  // epilogue warps that share a row: each EW columns
+    static constexpr int EW = BN / PARTS;
     static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 16 * STAGES + 64 + 8 * BN;
-    static_assert(BN % 128 == 0 && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
+    static_assert(BN % 32 == 0 && (EW == 32 || EW % 64 == 0) && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
     static_assert(!B_MN || BROWS % 64 == 0, "an MN-major box is 64 wide");
 };
 
@@ -95,12 +98,18 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 0x989680;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 0x989680;\n\t"
         "selp.b32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
     return ok != 0;
+}
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 // Waits for the phase of `parity` to end. False: the limit passed or another role gave up.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const GemmArgs &g, volatile unsigned *gave_up) {
@@ -115,6 +124,34 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const G
         }
     }
     return true;
+}
+
+// The same, without telling: a wait that passes the limit sets the flag (a shared-memory address) and the error
+// word and returns; once the flag is set, every wait returns after one try.
+__device__ __forceinline__ void mbar_wait_or_flag(uint32_t bar, uint32_t parity, const GemmArgs &g, uint32_t flag) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t.reg .u64 t0, t;\n\t.reg .u32 f;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+        "@p bra DONE;\n\t"
+        "mov.u64 t0, %%globaltimer;\n\t"
+        "AGAIN:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1, 0x989680;\n\t"
+        "@p bra DONE;\n\t"
+        "ld.volatile.shared.u32 f, [%3];\n\t"
+        "setp.ne.u32 p, f, 0;\n\t"
+        "@p bra DONE;\n\t"
+        "mov.u64 t, %%globaltimer;\n\t"
+        "sub.u64 t, t, t0;\n\t"
+        "setp.le.u64 p, t, %2;\n\t"
+        "@p bra AGAIN;\n\t"
+        "mov.u32 f, 1;\n\t"
+        "st.volatile.shared.u32 [%3], f;\n\t"
+        "red.global.or.b32 [%4], %5;\n\t"
+        "DONE:\n\t"
+        "}" ::"r"(bar),
+        "r"(parity), "l"(g.wait_ns), "r"(flag), "l"(g.error_word), "r"(DEVERR_WAIT_GEMM)
+        : "memory");
 }
 
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
@@ -268,6 +305,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const uint32_t full = bars, empty = bars + 8 * S, acc_full = bars + 16 * S, acc_empty = acc_full + 16;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 16 * S + 32);
     volatile unsigned *gave_up = reinterpret_cast<volatile unsigned *>(tail + 16 * S + 36);
+    const uint32_t flag = bars + 16 * S + 36;  // gave_up's address
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CTAS == 2 ? cluster_rank() : 0u;
 
@@ -278,7 +316,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + 8 * b, 1);
-            mbar_init(acc_empty + 8 * b, kEpilogueWarps * CTAS);
+            mbar_init(acc_empty + 8 * b, 4 * C::PARTS * CTAS);
         }
         *gave_up = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -296,22 +334,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
     if (warp == 0 && lane == 0) {
         // loads
-        int it = 0;
+        int s = 0, it = 0;
+        uint32_t phase = 1;
         bool ok = true;
         for (int t = first; ok && t < tiles; t += step) {
             int mt, nt;
             tile_at(g, m_tiles, t, mt, nt);
             const int am = mt * C::TM + (int)rank * C::BM, bn = nt * C::BN + (int)rank * C::BROWS;
             for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                const int s = it % S;
-                if (!mbar_wait(empty + 8 * s, ((it / S) & 1) ^ 1, g, gave_up)) {
+                if (!mbar_wait(empty + 8 * s, phase, g, gave_up)) {
                     ok = false;
                     break;
                 }
                 const uint32_t a_at = base + s * C::STAGE, b_at = a_at + C::A_BYTES;
                 const uint32_t bar = CTAS == 2 ? map_rank(full + 8 * s, 0) : full + 8 * s;
-                if (rank == 0) mbar_expect(full + 8 * s, C::STAGE * CTAS);
                 const int k0 = kb * kBlockK;
+                if (rank == 0) mbar_expect(full + 8 * s, g.stage_bytes * CTAS);
                 if constexpr (C::A_MN) {
 #pragma unroll
                     for (int c = 0; c < C::BM / 64; ++c) tma_load<CTAS>(a_at + c * 8192, &map_a, am + c * 64, k0, bar);
@@ -325,44 +363,53 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 } else {
                     tma_load<CTAS>(b_at, &map_b, k0, bn, bar);
                 }
+                if (++s == S) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
         }
         // the last products still read (and their commits still arrive at) these stages
         for (int j = it > S ? it - S : 0; ok && j < it; ++j)
             if (!mbar_wait(empty + 8 * (j % S), (j / S) & 1, g, gave_up)) ok = false;
-        // giving up: the copies in flight still land in this pair's shared memory (each try sleeps up to 10 ms)
+        // giving up: the copies in flight still land in this pair's shared memory (bounded: 2^20 tries each)
         if (!ok && rank == 0)
             for (int j = it > S ? it - S : 0; j < it; ++j)
-                for (int tries = 0; tries < 20 && !mbar_try(full + 8 * (j % S), (j / S) & 1); ++tries) {}
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        // products
-        int it = 0, n = 0;
-        bool ok = true;
-        for (int t = first; ok && t < tiles; t += step, ++n) {
+                for (int tries = 0; tries < (1 << 20) && !mbar_try(full + 8 * (j % S), (j / S) & 1); ++tries) {}
+    } else if (warp == 1 && rank == 0) {
+        // Products. The warp runs the loop whole, with waits that return nothing, so that what the instructions take
+        // stays in uniform registers; one lane issues (a commit covers what its own thread issued). After a wait
+        // that gave up the loop runs to its end on whatever the stages hold.
+        const bool issues = elect_one();
+        int s = 0, n = 0;
+        uint32_t phase = 0;
+        for (int t = first; t < tiles; t += step, ++n) {
             const int b = n & 1;
-            if (!mbar_wait(acc_empty + 8 * b, ((n >> 1) & 1) ^ 1, g, gave_up)) break;
+            mbar_wait_or_flag(acc_empty + 8 * b, ((n >> 1) & 1) ^ 1, g, flag);
             fence_after();
             const uint32_t d = tmem + b * C::BN;
-            for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                const int s = it % S;
-                if (!mbar_wait(full + 8 * s, (it / S) & 1, g, gave_up)) {
-                    ok = false;
-                    break;
-                }
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                mbar_wait_or_flag(full + 8 * s, phase, g, flag);
                 fence_after();
                 const uint32_t a_at = base + s * C::STAGE, b_at = a_at + C::A_BYTES;
                 const uint64_t da = smem_desc(a_at, C::A_MN ? 8192u : 16u), db = smem_desc(b_at, C::B_MN ? 8192u : 16u);
+                if (issues) {
 #pragma unroll
-                for (int k = 0; k < kBlockK / 16; ++k)  // 16 k: 32 bytes of a K-major row, 16 rows MN-major
-                    mma<CTAS>(d, da + (uint64_t)(k * (C::A_MN ? 2048 : 32) >> 4),
-                              db + (uint64_t)(k * (C::B_MN ? 2048 : 32) >> 4), g.idesc, (kb | k) != 0);
-                commit<CTAS>(empty + 8 * s);
+                    for (int k = 0; k < kBlockK / 16; ++k)  // 16 k: 32 bytes of a K-major row, 16 rows MN-major
+                        mma<CTAS>(d, da + (uint64_t)(k * (C::A_MN ? 2048 : 32) >> 4),
+                                  db + (uint64_t)(k * (C::B_MN ? 2048 : 32) >> 4), g.idesc, (kb | k) != 0);
+                    commit<CTAS>(empty + 8 * s);
+                }
+                if (++s == S) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
-            if (ok) commit<CTAS>(acc_full + 8 * b);
+            if (issues) commit<CTAS>(acc_full + 8 * b);
         }
     } else if (warp >= 4) {
         // epilogue: a warp reads its quarter of the tensor memory's lanes (a lane a row) and half of the columns
-        constexpr int EW = C::BN / 2;
+        constexpr int EW = C::EW;
         const int w = warp & 3, half = (warp - 4) >> 2;
         float *bias = reinterpret_cast<float *>(tail + 16 * S + 64);  // [2][BN]
         int n = 0;
@@ -385,13 +432,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const float *tile_bias = bias + b * C::BN + half * EW;
             // a warp that gave up goes on to the barriers, which the other warps may still wait at
             if (!failed) failed = !__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b, (n >> 1) & 1, g, gave_up));
-            if (failed) continue;
+            if (failed || half >= C::PARTS) continue;
             fence_after();
             const uint32_t at = tmem + ((uint32_t)(w * 32) << 16) + b * C::BN + half * EW;
 #pragma unroll 1
             for (int c = 0; c < EW; c += 64) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < (EW < 64 ? 1 : 2); ++h) {
                     const int64_t col = col0 + c + 32 * h;
                     uint32_t r[32];
                     __syncwarp();  // the loads are the whole warp's
@@ -403,7 +450,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
                         for (int j = 0; j < 32; ++j) r[j] = 0u;
                     }
-                    if (h == 1 && c + 64 >= EW) {  // all read: the next products may overwrite the accumulators
+                    if (c + 32 * (h + 1) >= EW) {  // all read: the next products may overwrite the accumulators
                         fence_before();
                         __syncwarp();
                         if (lane == 0)
@@ -426,6 +473,37 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (warp == 2) tmem_free<CTAS>(tmem, C::TMEM_COLS);
 }
 
+// Which tiles a product takes. A CTA's time is its k blocks times what one costs: bound by bringing in the
+// operands (an SM takes about 140 bytes a nanosecond), by the products from 256 columns on. Measured, ns a
+// block: pair 256x256 285, pair 256x128 180, 128x128 240, 128x64 180, 128x32 of few rows 120; then the
+// epilogue of the last tile. The cheapest by waves * blocks wins: few large tiles leave SMs idle, many small
+// ones bring the operands in more often. [1024,4096]x[4096,4096]^T: 128x128 37 us, pair 256x256 23 us;
+// [64,4096]x[4096,4096]^T: 128x128 20 us, 128x32 9 us.
+struct Tiles {
+    int ctas, bn, ew;  // ew: columns of an epilogue thread
+};
+inline Tiles pick_tiles(int64_t m, int64_t n, int64_t k, bool mn_major) {
+    struct Choice {
+        int ctas, bn, block_ns, tail_ns;
+    };
+    constexpr Choice all[] = {{2, 256, 285, 2500}, {2, 128, 180, 1600}, {1, 128, 240, 1600}, {1, 64, 180, 1400}, {1, 32, 120, 1000}};
+    const int64_t blocks = (k + kBlockK - 1) / kBlockK;
+    Tiles best{1, 128, 64};
+    int64_t least = INT64_MAX;
+    for (const Choice &c : all) {
+        if (c.ctas == 2 && m <= 128) continue;                 // half of each pair's rows would be empty
+        if (c.bn == 32 && (mn_major || m > 128)) continue;     // an MN-major box is 64 wide
+        const int64_t tiles = (m + 128 * c.ctas - 1) / (128 * c.ctas) * ((n + c.bn - 1) / c.bn);
+        const int64_t slots = 148 / c.ctas, waves = (tiles + slots - 1) / slots;
+        const int64_t cost = waves * blocks * c.block_ns + c.tail_ns;
+        if (cost < least) {
+            least = cost;
+            best = {c.ctas, c.bn, c.bn >= 128 ? c.bn / 2 : c.bn};
+        }
+    }
+    return best;
+}
+
 // Launches the product of a and b (already TMA-ready). With m_dev / k_dev, m and k are what they may reach.
 template <class C, class Epi>
 dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k, const Epi &epi,
@@ -438,8 +516,11 @@ dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m,
         opted[ds->device].store(1, std::memory_order_release);
     }
     CUtensorMap ma, mb;
+    // few rows: no more of A is brought in than there is (the tile's other rows hold what the memory held: their
+    // products are never looked at)
+    const int a_rows = !C::A_MN && C::CTAS == 1 && m < C::BM ? (int)((m + 7) / 8 * 8) : C::BM;
     if (C::A_MN) DNB_TRY(make_map(&ma, a.p, m, k, a.ld, 64, dtype, what));
-    else DNB_TRY(make_map(&ma, a.p, k, m, a.ld, C::BM, dtype, what));
+    else DNB_TRY(make_map(&ma, a.p, k, m, a.ld, a_rows, dtype, what));
     if (C::B_MN) DNB_TRY(make_map(&mb, b.p, n, k, b.ld, 64, dtype, what));
     else DNB_TRY(make_map(&mb, b.p, k, n, b.ld, C::BROWS, dtype, what));
     GemmArgs g;
@@ -452,6 +533,7 @@ dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m,
     g.n_tiles = (int)nt;
     g.k_blocks = (int)((k + kBlockK - 1) / kBlockK);
     g.band = 8;
+    g.stage_bytes = (unsigned)(a_rows * kBlockK * 2 + C::B_BYTES);
     g.m_dev = m_dev;
     g.k_dev = k_dev;
     // fp32 accumulators; operand type; majors; n / 8; m / 16

@@ -92,7 +92,7 @@ struct EpiStats {
     float2 *part;             // [tile][m]
     float *at_label;          // [m]
     int64_t m, n;
-    int bn;  // columns of a thread's part: half a tile
+    int bn;  // columns of a thread's part of a tile
 
     struct State {
         float top, sum;
@@ -335,6 +335,20 @@ __global__ void __launch_bounds__(256) k_delta_sums(const float *sums, const int
     }
 }
 
+// The tiles of the two products whose results stay in the epilogue: those of pick_tiles, in three of its shapes.
+Tiles xent_tiles(int64_t m, int64_t n, int64_t k) {
+    Tiles t = pick_tiles(m, n, k, true);
+    if (t.ctas == 2 && t.bn == 128) t = {1, 128, 64};
+    return t;
+}
+template <class Epi>
+dnb_status xent_product(const Tiles &t, const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k,
+                        const Epi &e, const DeviceState *ds, cudaStream_t s, const char *what, const int *m_dev) {
+    if (t.ctas == 2) return launch_gemm<GemmCfg<2, 256, false, false>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev);
+    if (t.bn == 64) return launch_gemm<GemmCfg<1, 64, false, false>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev);
+    return launch_gemm<GemmCfg<1, 128, false, false>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev);
+}
+
 // ---- the caller's workspace ----
 
 // Squeezing out padding rows pays from a few tiles of rows on: below, a forward takes every row.
@@ -346,14 +360,14 @@ struct FwdSpace {
     float *at_label;
     int *rows, *count;
     int64_t tiles;
-    int bn;
+    Tiles shape;
     size_t total;
 };
 FwdSpace fwd_space(void *ws, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t m, int64_t k, int64_t n) {
     Carver c(ws);
     FwdSpace f{};
-    f.bn = (big_tiles(m, n) ? 256 : 128) / 2;  // the epilogue's half tiles
-    f.tiles = (n + f.bn - 1) / f.bn;
+    f.shape = xent_tiles(m, n, k);
+    f.tiles = (n + f.shape.ew - 1) / f.shape.ew;
     f.part = static_cast<float2 *>(c.take(f.tiles * m * 8));
     f.at_label = static_cast<float *>(c.take(m * 4));
     if (squeezes(m)) {
@@ -454,12 +468,8 @@ dnb_status dnb_connected_xent_forward(const void *x, int64_t ldx, const void *w,
     DNB_TRY(pack_rows({x, ldx, f.x, batch, inputs}, {w, ldw, f.w, classes, inputs}, dtype, g, ds, s, what));
     if (f.x) a = {f.x, packed_ld(inputs)};
     if (f.w) b = {f.w, packed_ld(inputs)};
-    EpiStats e{biases, labels, f.rows, f.count, f.part, f.at_label, batch, classes, f.bn};
-    const dnb_status st =
-        f.bn == 128
-            ? launch_gemm<GemmCfg<2, 256, false, false>>(a, b, dtype, batch, classes, inputs, e, ds, s, what, f.count)
-            : launch_gemm<GemmCfg<1, 128, false, false>>(a, b, dtype, batch, classes, inputs, e, ds, s, what, f.count);
-    DNB_TRY(st);
+    EpiStats e{biases, labels, f.rows, f.count, f.part, f.at_label, batch, classes, f.shape.ew};
+    DNB_TRY(xent_product(f.shape, a, b, dtype, batch, classes, inputs, e, ds, s, what, f.count));
     k_xent_close<<<(unsigned)((batch + 31) / 32), 1024, 0, s>>>(f.part, f.at_label, labels, f.rows, f.count, batch,
                                                                f.tiles, classes, loss, lse);
     return after_launch(s, what);
@@ -562,11 +572,7 @@ dnb_status dnb_connected_xent_backward(const void *x, int64_t ldx, const void *w
         e.sums = bias_updates ? f.sums : nullptr;
         e.scale = scale;
         e.dtype = dtype;
-        const dnb_status st =
-            big_tiles(batch, n)
-                ? launch_gemm<GemmCfg<2, 256, false, false>>(xp, wq, dtype, rows, n, inputs, e, ds, s, what, f.count)
-                : launch_gemm<GemmCfg<1, 128, false, false>>(xp, wq, dtype, rows, n, inputs, e, ds, s, what, f.count);
-        DNB_TRY(st);
+        DNB_TRY(xent_product(xent_tiles(batch, n, inputs), xp, wq, dtype, rows, n, inputs, e, ds, s, what, f.count));
         if (bias_updates) {
             k_delta_sums<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(f.sums, f.count, n, f.piece, bias_updates + c0, add_w);
             DNB_TRY(after_launch(s, what));
@@ -581,7 +587,7 @@ dnb_status dnb_connected_xent_backward(const void *x, int64_t ldx, const void *w
             o.row_factor = row_scales;
             o.rows = f.rows;
             o.m_dev = f.count;
-            const dnb_status sx = product<false, true>(d, wq, dtype, rows, inputs, n, o, ds, s, what, f.count);
+            const dnb_status sx = product(false, true, d, wq, dtype, rows, inputs, n, o, ds, s, what, f.count);
             DNB_TRY(sx);
         }
         if (weight_updates) {
@@ -593,7 +599,7 @@ dnb_status dnb_connected_xent_backward(const void *x, int64_t ldx, const void *w
                 o.alpha = 1.0f;
                 o.alpha_dev = f.meta + 1;
             }
-            const dnb_status sw = product<true, true>(d, xs, dtype, n, inputs, rows, o, ds, s, what, nullptr, f.count);
+            const dnb_status sw = product(true, true, d, xs, dtype, n, inputs, rows, o, ds, s, what, nullptr, f.count);
             DNB_TRY(sw);
         }
     }
