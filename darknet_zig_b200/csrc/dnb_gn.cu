@@ -317,7 +317,7 @@ dnb_status dnb_gn_act_forward_workspace(const void *x, const void *y, int dtype,
     *bytes = 0;
     if (batch == 0 || spatial == 0) return DNB_OK;
     const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y);
-    const GnPlan p = gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, 1, false);
+    const GnPlan p = gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, false);
     if (p.stream) *bytes = (size_t)(batch * groups * p.chunks) * 8;
     return DNB_OK;
 }
@@ -337,7 +337,7 @@ dnb_status dnb_gn_act_forward(const void *x, void *y, int dtype, int64_t batch, 
     if ((x != y && overlaps(x, bytes, y, bytes)) || overlaps(mean, st, rstd, st) || overlaps(mean, st, y, bytes) ||
         overlaps(rstd, st, y, bytes) || overlaps(mean, st, x, bytes) || overlaps(rstd, st, x, bytes))
         return fail(DNB_ERR_INVALID, "%s: overlapping tensors", what);
-    const GnPlan p = gn_plan(batch, spatial, filters, groups, e, align, 1, false);
+    const GnPlan p = gn_plan(batch, spatial, filters, groups, e, align, false);
     const size_t need = p.stream ? (size_t)(batch * groups * p.chunks) * 8 : 0;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(DNB_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what, need,

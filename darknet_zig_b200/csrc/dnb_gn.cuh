@@ -36,6 +36,9 @@ struct GnPlan {
 
 constexpr size_t kGnSmemTarget = 112 * 1024;  // two CTAs an SM
 constexpr size_t kGnSmemMax = 200 * 1024;
+// Backward: bytes of one tensor's rows of a CTA that the L2 cache keeps from the sums to the outputs (two or
+// three tensors, some 400 CTAs at a time: 60 MB of its 126).
+constexpr size_t kGnReread = 64 * 1024;
 constexpr size_t kGnStreamBytes = 64 * 1024;  // a streaming chunk's inputs
 constexpr int kGnMaxCluster = 8;
 constexpr int64_t kGnMaxGroup = 4096;         // channels of a group: a row of them, with the partials, fits an SM
@@ -62,11 +65,9 @@ inline int64_t gcd64(int64_t a, int64_t b) {
     return a;
 }
 
-// tensors: planes of vectors held in shared memory (1 forward, 2 or 3 backward); align: the OR of the tensors'
-// addresses. Whether a unit streams, and how, does not depend on `tensors`: the backward's workspace is asked for
-// before its activation is known.
+// align: the OR of the tensors' addresses.
 inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t groups, int64_t esize, uintptr_t align,
-                      int tensors, bool backward) {
+                      bool backward) {
     constexpr int sms = 148;  // a B200's; the plan must not depend on the current device, for the workspace's size
     GnPlan p;
     const int64_t cg = filters / groups;
@@ -86,30 +87,33 @@ inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t g
            units_of(cap(2 * per)) >= 2 * sms)
         per = cap(2 * per);
     // rows narrower than 64 bytes rather than a second read of the inputs
-    const int most_planes = backward ? 3 : 1;
-    if (slab_of(per, (spatial + kGnMaxCluster - 1) / kGnMaxCluster) * most_planes > kGnSmemMax && step < per)
+    // (backward: rows that the L2 cache would not keep until they are read again)
+    if (slab_of(per, (spatial + kGnMaxCluster - 1) / kGnMaxCluster) > (backward ? kGnReread : kGnSmemMax) && step < per)
         per = cap(step);
     p.cb = per * cg;
     p.nu = (groups + per - 1) / per;
-    auto sizes = [&](size_t slabs) {
+    auto sizes = [&](bool held) {
         const int64_t v = p.cb / n, wide = p.threads > v ? p.threads : v;
         // forward: two floats a thread and vector (or channel), four floats a group;
         // backward: two floats a channel of a thread, two a thread (slices), two a channel, two a group
         p.part = (size_t)(((backward || !p.uni ? wide * n : wide) + 3) / 4 * 4);
-        p.smem = p.slab * slabs + p.part * 8 + 64;
+        p.smem = (held ? p.slab : 0) + p.part * 8 + 64;
         p.smem += backward ? (size_t)p.threads * 8 + (size_t)p.cb * 8 + (size_t)per * 8 : (size_t)per * 16;
         p.smem += (size_t)p.cb * 8;  // scales and biases
     };
-    auto shape = [&](int q, int planes) {
+    auto shape = [&](int q) {
         p.cluster = q;
         p.rows = (spatial + q - 1) / q;
         p.slab = slab_of(per, p.rows);
         // a warp's fixed work (places, reductions) is that of a dozen vectors: no more threads than get those
-        p.threads = p.rows * (p.cb / n) >= 12 * 512 ? 512 : 256;
-        sizes((size_t)planes);
+        p.threads = !backward && p.rows * (p.cb / n) >= 12 * 512 ? 512 : 256;
+        sizes(!backward);
     };
-    shape(kGnMaxCluster, most_planes);
-    if (p.smem > kGnSmemMax) {
+    auto too_big = [&] { return backward ? p.slab > kGnReread : p.smem > kGnSmemTarget; };
+    int q = 1;
+    shape(q);
+    while (q < kGnMaxCluster && too_big()) shape(q *= 2);
+    if (backward ? p.slab > kGnReread : p.smem > kGnSmemMax) {
         p.stream = true;
         p.cluster = 1;
         p.rows = (int64_t)(kGnStreamBytes / (size_t)(p.cb * esize * (backward ? 2 : 1)));
@@ -117,14 +121,11 @@ inline GnPlan gn_plan(int64_t batch, int64_t spatial, int64_t filters, int64_t g
         p.chunks = (spatial + p.rows - 1) / p.rows;
         p.slab = 0;
         p.threads = 256;
-        sizes(0);
+        sizes(false);
         return p;
     }
-    int q = 1;
-    shape(q, tensors);
-    while (q < kGnMaxCluster && p.smem > kGnSmemTarget) shape(q *= 2, tensors);
-    // few units: more CTAs for each, while a CTA keeps 8 KB
-    while (q < kGnMaxCluster && units_of(per) * q < sms && p.slab * tensors > 16 * 1024) shape(q *= 2, tensors);
+    // few units: more CTAs for each, while a CTA keeps 8 KB (backward: of each tensor)
+    while (q < kGnMaxCluster && units_of(per) * q < sms && p.slab > 16 * 1024) shape(q *= 2);
     return p;
 }
 

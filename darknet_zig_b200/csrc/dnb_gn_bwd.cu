@@ -25,7 +25,7 @@ struct GnBwd {
     int64_t spatial, filters, groups, cg, cb, nu, rows, chunks;
     double inv_count;  // 1 / n
     int act, cluster, unit_groups;
-    unsigned slab, part, planes;
+    unsigned part;
 };
 
 // The activation's gradient times delta for a pair, from the given output or the recomputed one (z: its
@@ -56,59 +56,6 @@ __device__ __forceinline__ void store_pairs(float *p, const float2 (&s)[(N + 1) 
 #pragma unroll
         for (int i = 0; i < N / 2; i += 2)
             *reinterpret_cast<float4 *>(p + 2 * i) = make_float4(s[i].x, s[i].y, s[i + 1].x, s[i + 1].y);
-}
-
-// Whether a thread leaves d in shared memory, in fp32, over the delta (and y) it came from, instead of forming
-// it again for dx: where forming it is dear (a logistic's special-function results bound the kernel) or takes
-// y. A 16-bit d fills two planes of vectors, delta's and y's (or a spare one): 6 bytes an element in place of
-// 4 and half the special-function work; [128,784,256] bf16 logistic 60 -> 47 us.
-template <int A, bool Y>
-constexpr bool kKeeps = Y || A == DNB_ACT_LOGISTIC || A == -1;
-// Planes of input vectors in shared memory: x, delta, and y or the second half of a 16-bit d.
-inline int planes_of(int act, bool y, int64_t esize) {
-    const bool dear = act != DNB_ACT_LINEAR && act != DNB_ACT_LEAKY && act != DNB_ACT_RELU;
-    return y || (dear && esize == 2) ? 3 : 2;
-}
-// d of a vector: fp32 in the vector's own place in the plane at p; of 16-bit types the first half there, the
-// second in the next plane.
-template <class T, int VB>
-__device__ __forceinline__ void keep_pairs(unsigned char *p, unsigned plane, const float2 (&d)[(VB / (int)sizeof(T) + 1) / 2]) {
-    if constexpr (VB == 16 && sizeof(T) == 2) {
-        *reinterpret_cast<float4 *>(p) = make_float4(d[0].x, d[0].y, d[1].x, d[1].y);
-        *reinterpret_cast<float4 *>(p + plane) = make_float4(d[2].x, d[2].y, d[3].x, d[3].y);
-    } else if constexpr (VB == 16) {
-        *reinterpret_cast<float4 *>(p) = make_float4(d[0].x, d[0].y, d[1].x, d[1].y);
-    } else if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float *>(p) = d[0].x;
-    } else if constexpr (VB == 4) {
-        *reinterpret_cast<float *>(p) = d[0].x;
-        *reinterpret_cast<float *>(p + plane) = d[0].y;
-    } else {  // two bytes each
-        const uint32_t w = __float_as_uint(d[0].x);
-        *reinterpret_cast<uint16_t *>(p) = (uint16_t)w;
-        *reinterpret_cast<uint16_t *>(p + plane) = (uint16_t)(w >> 16);
-    }
-}
-template <class T, int VB>
-__device__ __forceinline__ void kept_pairs(const unsigned char *p, unsigned plane, float2 (&d)[(VB / (int)sizeof(T) + 1) / 2]) {
-    if constexpr (VB == 16) {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        d[0] = make_float2(v.x, v.y);
-        d[1] = make_float2(v.z, v.w);
-        if constexpr (sizeof(T) == 2) {
-            const float4 u = *reinterpret_cast<const float4 *>(p + plane);
-            d[2] = make_float2(u.x, u.y);
-            d[3] = make_float2(u.z, u.w);
-        }
-    } else if constexpr (sizeof(T) == 4) {
-        d[0] = make_float2(*reinterpret_cast<const float *>(p), 0.0f);
-    } else if constexpr (VB == 4) {
-        d[0] = make_float2(*reinterpret_cast<const float *>(p), *reinterpret_cast<const float *>(p + plane));
-    } else {
-        const uint32_t w = *reinterpret_cast<const uint16_t *>(p) |
-                           (uint32_t) * reinterpret_cast<const uint16_t *>(p + plane) << 16;
-        d[0] = make_float2(__uint_as_float(w), 0.0f);
-    }
 }
 
 // The group's (c1, c2) for a vector's channels.
@@ -143,16 +90,13 @@ __device__ __forceinline__ void dx_of(float2 (&fx)[P], const float2 (&fd)[P], co
 }
 
 template <class T, int VB, int A, bool Y, bool UNI, bool STREAM>
-__global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a) {
+__global__ void __launch_bounds__(256, 3) k_gn_bwd(const __grid_constant__ GnBwd a) {
     using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
     constexpr int N = V::N, P = V::P;
     extern __shared__ __align__(16) unsigned char smem[];
     const Place p = place_of(a, STREAM ? (unsigned)a.chunks : (unsigned)a.cluster);
-    constexpr bool KEEP = kKeeps<A, Y>;
-    T *sx = reinterpret_cast<T *>(smem), *sd = reinterpret_cast<T *>(smem + a.slab),
-      *sy = reinterpret_cast<T *>(smem + 2 * a.slab);
-    float *part = reinterpret_cast<float *>(smem + (STREAM ? 0u : a.planes * a.slab));
+    float *part = reinterpret_cast<float *>(smem);
     float2 *slices = reinterpret_cast<float2 *>(part + 2 * a.part);
     const int nt = blockDim.x;
     float2 *ch = slices + nt;                                    // the channels' sums
@@ -163,67 +107,57 @@ __global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a)
     const bool on = rl < rl_n;
     const int64_t base = (p.b * a.spatial + p.r0) * a.filters + p.c0, g0 = p.b * a.groups + p.g0;
     const int64_t pitch = a.filters * rl_n;
-    const int cg = (int)a.cg, srow = rl_n * p.cb;
-    (void)sy;
+    const int cg = (int)a.cg;
 
     gn_stage_params(sc, a.scales, a.biases, p);
-    if constexpr (!STREAM) {
-        for (int col = col0; col < v; col += vp) {
-            if (!on) break;
-            const int64_t at = base + (int64_t)rl * a.filters + (int64_t)col * N;
-            const T *x = static_cast<const T *>(a.x) + at, *delta = static_cast<const T *>(a.delta) + at;
-            const T *y = Y ? static_cast<const T *>(a.y) + at : nullptr;
-            int in = rl * p.cb + col * N;
-#pragma unroll 2
-            for (int r = rl; r < p.nr; r += rl_n) {
-                gn_copy<VB>(sx + in, x);
-                gn_copy<VB>(sd + in, delta);
-                if constexpr (Y) {
-                    gn_copy<VB>(sy + in, y);
-                    y += pitch;
-                }
-                x += pitch;
-                delta += pitch;
-                in += srow;
-            }
-        }
-    }
     __syncthreads();
-    if constexpr (!STREAM) gn_arrived();
 
     for (int col = col0; col < v; col += vp) {
         if (!on) break;
         Affine<N, UNI> k;
         k.load(col, cg, a.mean + g0, a.rstd + g0, sc, bi);
         float2 s0[P] = {}, s1[P] = {};
-        const int64_t at = base + (int64_t)rl * a.filters + (int64_t)col * N, in = rl * p.cb + col * N;
-        const T *x = STREAM ? static_cast<const T *>(a.x) + at : sx + in;
-        const T *delta = STREAM ? static_cast<const T *>(a.delta) + at : sd + in;
-        const T *y = !Y ? nullptr : STREAM ? static_cast<const T *>(a.y) + at : sy + in;
-        const int64_t step = STREAM ? pitch : srow;
-        unsigned char *keep = reinterpret_cast<unsigned char *>(sd + in);
-#pragma unroll 2
-        for (int r = rl; r < p.nr; r += rl_n) {
+        const int64_t at = base + (int64_t)rl * a.filters + (int64_t)col * N;
+        const T *x = static_cast<const T *>(a.x) + at, *delta = static_cast<const T *>(a.delta) + at;
+        const T *y = Y ? static_cast<const T *>(a.y) + at : nullptr;
+        auto add = [&](Raw rx, Raw rd, Raw ry) {
             float2 fx[P], fd[P], fy[P] = {};
-            V::unpack(*reinterpret_cast<const Raw *>(x), fx);
-            V::unpack(*reinterpret_cast<const Raw *>(delta), fd);
-            if constexpr (Y) {
-                V::unpack(*reinterpret_cast<const Raw *>(y), fy);
-                y += step;
-            }
-            x += step;
-            delta += step;
+            V::unpack(rx, fx);
+            V::unpack(rd, fd);
+            if constexpr (Y) V::unpack(ry, fy);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const float2 z = Y ? fy[i] : k.z(fx[i], i);
-                fd[i] = through<A, Y>(fd[i], fy[i], z, a.act);
-                s0[i] = __fadd2_rn(s0[i], fd[i]);
-                s1[i] = __ffma2_rn(fd[i], __fadd2_rn(fx[i], k.m[UNI ? 0 : i]), s1[i]);
+                const float2 d = through<A, Y>(fd[i], fy[i], z, a.act);
+                s0[i] = __fadd2_rn(s0[i], d);
+                s1[i] = __ffma2_rn(d, __fadd2_rn(fx[i], k.m[UNI ? 0 : i]), s1[i]);
             }
-            if constexpr (!STREAM && KEEP) {
-                keep_pairs<T, VB>(keep, a.slab, fd);
-                keep += step * (int)sizeof(T);
+        };
+        constexpr int U = Y ? 2 : 4;
+        int r = rl;
+        for (; r + (U - 1) * rl_n < p.nr; r += U * rl_n) {
+            Raw rx[U], rd[U], ry[U] = {};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                rx[u] = *reinterpret_cast<const Raw *>(x + u * pitch);
+                rd[u] = *reinterpret_cast<const Raw *>(delta + u * pitch);
+                if constexpr (Y) ry[u] = *reinterpret_cast<const Raw *>(y + u * pitch);
             }
+            x += U * pitch;
+            delta += U * pitch;
+            if constexpr (Y) y += U * pitch;
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(rx[u], rd[u], ry[u]);
+        }
+        for (; r < p.nr; r += rl_n) {
+            Raw ry{};
+            if constexpr (Y) {
+                ry = *reinterpret_cast<const Raw *>(y);
+                y += pitch;
+            }
+            add(*reinterpret_cast<const Raw *>(x), *reinterpret_cast<const Raw *>(delta), ry);
+            x += pitch;
+            delta += pitch;
         }
         if constexpr (UNI) {
 #pragma unroll
@@ -320,22 +254,38 @@ __global__ void __launch_bounds__(512) k_gn_bwd(const __grid_constant__ GnBwd a)
         k.load(col, cg, a.mean + g0, a.rstd + g0, sc, bi);
         float2 c1[UNI ? 1 : P], c2[UNI ? 1 : P];
         load_moments<N, UNI>(col, cg, mo, c1, c2);
-        T *dx = static_cast<T *>(a.dx) + base + (int64_t)rl * a.filters + (int64_t)col * N;
-        int in = rl * p.cb + col * N;
-#pragma unroll 2
-        for (int r = rl; r < p.nr; r += rl_n) {
+        // dx may be delta: a batch of rows is read before the first of it is written
+        int64_t at = base + (int64_t)rl * a.filters + (int64_t)col * N;
+        const T *x = static_cast<const T *>(a.x), *delta = static_cast<const T *>(a.delta),
+                *y = static_cast<const T *>(a.y);
+        T *dx = static_cast<T *>(a.dx);
+        auto give = [&](Raw rx, Raw rd, Raw ry, int64_t to) {
             float2 fx[P], fd[P], fy[P] = {};
-            V::unpack(*reinterpret_cast<const Raw *>(sx + in), fx);
-            if constexpr (KEEP) {
-                kept_pairs<T, VB>(reinterpret_cast<const unsigned char *>(sd + in), a.slab, fd);
-                dx_of<P, DNB_ACT_LINEAR, false, UNI>(fx, fd, fy, k, c1, c2, a.act);
-            } else {
-                V::unpack(*reinterpret_cast<const Raw *>(sd + in), fd);
-                dx_of<P, A, Y, UNI>(fx, fd, fy, k, c1, c2, a.act);
+            V::unpack(rx, fx);
+            V::unpack(rd, fd);
+            if constexpr (Y) V::unpack(ry, fy);
+            dx_of<P, A, Y, UNI>(fx, fd, fy, k, c1, c2, a.act);
+            *reinterpret_cast<Raw *>(dx + to) = V::pack(fx);
+        };
+        constexpr int U = Y ? 2 : 4;
+        int r = rl;
+        for (; r + (U - 1) * rl_n < p.nr; r += U * rl_n) {
+            Raw rx[U], rd[U], ry[U] = {};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                rx[u] = *reinterpret_cast<const Raw *>(x + at + u * pitch);
+                rd[u] = *reinterpret_cast<const Raw *>(delta + at + u * pitch);
+                if constexpr (Y) ry[u] = *reinterpret_cast<const Raw *>(y + at + u * pitch);
             }
-            in += srow;
-            *reinterpret_cast<Raw *>(dx) = V::pack(fx);
-            dx += pitch;
+#pragma unroll
+            for (int u = 0; u < U; ++u) give(rx[u], rd[u], ry[u], at + u * pitch);
+            at += U * pitch;
+        }
+        for (; r < p.nr; r += rl_n) {
+            Raw ry{};
+            if constexpr (Y) ry = *reinterpret_cast<const Raw *>(y + at);
+            give(*reinterpret_cast<const Raw *>(x + at), *reinterpret_cast<const Raw *>(delta + at), ry, at);
+            at += pitch;
         }
     }
     if (q_n > 1) gn_cluster_wait();
@@ -447,10 +397,10 @@ BwdSpace space_of(const GnPlan &p, int64_t batch, int64_t filters, int64_t group
 }
 
 GnPlan plan_bwd(const void *x, const void *y, const void *delta, const void *dx, int dtype, int64_t batch,
-                int64_t spatial, int64_t filters, int64_t groups, int planes = 3) {
+                int64_t spatial, int64_t filters, int64_t groups) {
     const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) |
                             reinterpret_cast<uintptr_t>(delta) | reinterpret_cast<uintptr_t>(dx);
-    return gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, planes, true);
+    return gn_plan(batch, spatial, filters, groups, dtype_size(dtype), align, true);
 }
 
 template <class T, int VB, int A, bool Y, bool UNI>
@@ -520,8 +470,7 @@ dnb_status dnb_gn_act_backward(const void *x, const void *y, const void *delta, 
         (dx != delta && overlaps(dx, bytes, delta, bytes)) || overlaps(bias_updates, fb, scale_updates, fb) ||
         overlaps(dx, bytes, bias_updates, fb) || overlaps(dx, bytes, scale_updates, fb))
         return fail(DNB_ERR_INVALID, "%s: overlapping tensors", what);
-    const int planes = planes_of(act, y != nullptr, e);
-    const GnPlan p = plan_bwd(x, y, delta, dx, dtype, batch, spatial, filters, groups, planes);
+    const GnPlan p = plan_bwd(x, y, delta, dx, dtype, batch, spatial, filters, groups);
     const BwdSpace w = space_of(p, batch, filters, groups);
     if (!workspace || workspace_bytes < w.total || !aligned16(workspace))
         return fail(DNB_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what, w.total,
@@ -552,9 +501,7 @@ dnb_status dnb_gn_act_backward(const void *x, const void *y, const void *delta, 
     a.act = act;
     a.cluster = p.cluster;
     a.unit_groups = (int)(p.cb / a.cg);
-    a.slab = (unsigned)p.slab;
     a.part = (unsigned)p.part;
-    a.planes = (unsigned)planes;
     auto with_y = [&]<class T, int VB, int A, bool UNI>() {
         return y ? run_bwd<T, VB, A, true, UNI>(a, p, batch, ds, s) : run_bwd<T, VB, A, false, UNI>(a, p, batch, ds, s);
     };
