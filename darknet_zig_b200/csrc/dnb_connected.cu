@@ -29,7 +29,7 @@ template <class T, int VB, int MB>
 __global__ void __launch_bounds__(256) k_rows(const __grid_constant__ RowsArgs a, int wpr) {
     using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
-    constexpr int N = V::N, P = V::P, U = MB == 1 ? 8 : 4;
+    constexpr int N = V::N, P = V::P, U = MB == 4 ? 2 : 4;
     __shared__ float red[8][MB];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, outs = 8 / wpr;
     const int64_t row = (int64_t)blockIdx.x * outs + warp / wpr;
@@ -90,12 +90,15 @@ __global__ void __launch_bounds__(256) k_rows(const __grid_constant__ RowsArgs a
 
 template <class T, int VB>
 dnb_status run_rows(const RowsArgs &a, cudaStream_t s, const char *what) {
+    // a warp an output from 4096 of them on; fewer are shared by more warps, while a lane keeps two vectors.
+    // [1,4096]x[4096,4096]^T: 1, 2 and 4 warps an output 5.9, 7.2 and 9.1 us; [1,4096]x[1000,4096]^T: 5.0, 3.8, 3.4
     int wpr = 1;
-    while (wpr < 8 && a.n * wpr < 8192 && a.k >= 512 * wpr) wpr *= 2;
+    while (wpr < 8 && a.n * wpr * 2 <= 4096 && a.k >= 512 * wpr) wpr *= 2;
     const int64_t outs = 8 / wpr, blocks = (a.n + outs - 1) / outs;
     if (blocks > 0x7fffffffll) return fail(DNB_ERR_UNSUPPORTED, "%s: too many outputs", what);
     if (a.m == 1) k_rows<T, VB, 1><<<dim3((unsigned)blocks, 1), 256, 0, s>>>(a, wpr);
-    else k_rows<T, VB, 2><<<dim3((unsigned)blocks, (unsigned)((a.m + 1) / 2)), 256, 0, s>>>(a, wpr);
+    else if (a.m == 2) k_rows<T, VB, 2><<<dim3((unsigned)blocks, 1), 256, 0, s>>>(a, wpr);
+    else k_rows<T, VB, 4><<<dim3((unsigned)blocks, (unsigned)((a.m + 3) / 4)), 256, 0, s>>>(a, wpr);
     return after_launch(s, what);
 }
 
@@ -109,39 +112,63 @@ struct DzArgs {
     int act, rows;    // rows of a chunk
 };
 
+// A block takes kDzRows rows of 64 vectors of columns: 4 row lanes, each with four rows on their way at a time
+// (dz may be delta, so that nothing is hoisted past a store by itself). Bound by memory: [8192,4096] bf16 with
+// an output, 201 MB, 50 us with one row lane of 256 vectors and 33 us so.
 template <class T, int VB, int A>
 __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
-    using V = Vec<T, VB>;
+    using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
-    constexpr int N = V::N;
-    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
-    if (c >= a.n) return;
+    constexpr int N = V::N, P = V::P, U = 4;
+    __shared__ float part[4][64 * N];
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + tx) * N;
     const int64_t r0 = (int64_t)blockIdx.y * a.rows, r1 = r0 + a.rows < a.m ? r0 + a.rows : a.m;
-    float sum[N] = {};
-#pragma unroll 4
-    for (int64_t r = r0; r < r1; ++r) {
-        float d[N];
-        V::unpack(*reinterpret_cast<const Raw *>(static_cast<const T *>(a.delta) + r * a.ldd + c), d);
-        if constexpr (A != DNB_ACT_LINEAR) {
-            float y[N];
-            V::unpack(*reinterpret_cast<const Raw *>(static_cast<const T *>(a.y) + r * a.ldy + c), y);
+    float2 sum[P] = {};
+    if (c < a.n) {
+        const T *delta = static_cast<const T *>(a.delta) + c, *y = static_cast<const T *>(a.y) + c;
+        T *dz = static_cast<T *>(a.dz), *copy = static_cast<T *>(a.copy);
+        for (int64_t r = r0 + ty; r < r1; r += 4 * U) {
+            Raw rd[U] = {}, ry[U] = {};
 #pragma unroll
-            for (int j = 0; j < N; ++j) d[j] *= act_grad<A>(y[j], a.act);
+            for (int u = 0; u < U; ++u) {
+                if (r + 4 * u >= r1) break;
+                rd[u] = *reinterpret_cast<const Raw *>(delta + (r + 4 * u) * a.ldd);
+                if constexpr (A != DNB_ACT_LINEAR) ry[u] = *reinterpret_cast<const Raw *>(y + (r + 4 * u) * a.ldy);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r + 4 * u >= r1) break;
+                float2 d[P];
+                V::unpack(rd[u], d);
+                if constexpr (A != DNB_ACT_LINEAR) {
+                    float2 f[P];
+                    V::unpack(ry[u], f);
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        d[i] = __fmul2_rn(d[i], make_float2(act_grad<A>(f[i].x, a.act), act_grad<A>(f[i].y, a.act)));
+                }
+                const Raw raw = V::pack(d);
+                if (dz) *reinterpret_cast<Raw *>(dz + (r + 4 * u) * a.lddz + c) = raw;
+                if (copy) *reinterpret_cast<Raw *>(copy + (r + 4 * u) * a.ld_copy + c) = raw;
+#pragma unroll
+                for (int i = 0; i < P; ++i) sum[i] = __fadd2_rn(sum[i], d[i]);
+            }
         }
-        const Raw raw = V::pack(d);
-        if (a.dz) *reinterpret_cast<Raw *>(static_cast<T *>(a.dz) + r * a.lddz + c) = raw;
-        if (a.copy) *reinterpret_cast<Raw *>(static_cast<T *>(a.copy) + r * a.ld_copy + c) = raw;
-#pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] += d[j];
     }
-    if (a.part)
+    if (!a.part) return;
 #pragma unroll
-        for (int j = 0; j < N; ++j) a.part[(int64_t)blockIdx.y * a.n + c + j] = sum[j];
+    for (int j = 0; j < N; ++j) part[ty][tx * N + j] = j & 1 ? sum[j / 2].y : sum[j / 2].x;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * N; i += 256) {
+        const int64_t col = (int64_t)blockIdx.x * (64 * N) + i;
+        if (col < a.n) a.part[(int64_t)blockIdx.y * a.n + col] = part[0][i] + part[1][i] + part[2][i] + part[3][i];
+    }
 }
 
 constexpr int kDzRows = 64;
 
-constexpr int64_t kFewRows = 2;  // [1 | 2 | 4 rows, 4096] x [4096, 4096]^T
+constexpr int64_t kFewRows = 4;  // [1 | 2 | 4 rows, 4096] x [4096, 4096]^T
 
 struct FwdSpace {
     void *x, *w;
@@ -219,7 +246,7 @@ dnb_status dnb_connected_act_forward(const void *x, int64_t ldx, const void *w, 
         RowsArgs a{x, w, residual, y, biases, ldx, ldw, ldr, ldy, batch, outputs, inputs, act, dtype};
         a.n = outputs;
         a.k = inputs;
-        if (batch > 2 * 65535) return fail(DNB_ERR_UNSUPPORTED, "%s: too many rows without inputs", what);
+        if (batch > 4 * 65535) return fail(DNB_ERR_UNSUPPORTED, "%s: too many rows without inputs", what);
         const uintptr_t al = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) |
                              (batch > 1 ? (uintptr_t)ldx * 2 : 0) | (outputs > 1 ? (uintptr_t)ldw * 2 : 0);
         return dispatch_dtype16(dtype, [&]<class T>() {
@@ -337,7 +364,7 @@ dnb_status dnb_connected_act_backward(const void *x, int64_t ldx, const void *w,
         const dnb_status st = dispatch_dtype16(dtype, [&]<class T>() {
             return dispatch_act(act, [&]<int A>() {
                 const int n = al % 16 == 0 ? 8 : 1;
-                const dim3 grid((unsigned)((outputs + 256 * n - 1) / (256 * n)), (unsigned)chunks);
+                const dim3 grid((unsigned)((outputs + 64 * n - 1) / (64 * n)), (unsigned)chunks);
                 if (n == 8) k_dz<T, 16, A><<<grid, 256, 0, s>>>(a);
                 else k_dz<T, 2, A><<<grid, 256, 0, s>>>(a);
                 return after_launch(s, what);
