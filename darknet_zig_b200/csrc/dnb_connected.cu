@@ -29,7 +29,7 @@ template <class T, int VB, int MB>
 __global__ void __launch_bounds__(256) k_rows(const __grid_constant__ RowsArgs a, int wpr) {
     using V = Pairs<T, VB>;
     using Raw = typename V::Raw;
-    constexpr int N = V::N, P = V::P, U = MB == 4 ? 2 : 4;
+    constexpr int N = V::N, P = V::P, U = 4;
     __shared__ float red[8][MB];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, outs = 8 / wpr;
     const int64_t row = (int64_t)blockIdx.x * outs + warp / wpr;
@@ -97,8 +97,7 @@ dnb_status run_rows(const RowsArgs &a, cudaStream_t s, const char *what) {
     const int64_t outs = 8 / wpr, blocks = (a.n + outs - 1) / outs;
     if (blocks > 0x7fffffffll) return fail(DNB_ERR_UNSUPPORTED, "%s: too many outputs", what);
     if (a.m == 1) k_rows<T, VB, 1><<<dim3((unsigned)blocks, 1), 256, 0, s>>>(a, wpr);
-    else if (a.m == 2) k_rows<T, VB, 2><<<dim3((unsigned)blocks, 1), 256, 0, s>>>(a, wpr);
-    else k_rows<T, VB, 4><<<dim3((unsigned)blocks, (unsigned)((a.m + 3) / 4)), 256, 0, s>>>(a, wpr);
+    else k_rows<T, VB, 2><<<dim3((unsigned)blocks, (unsigned)((a.m + 1) / 2)), 256, 0, s>>>(a, wpr);
     return after_launch(s, what);
 }
 
@@ -168,7 +167,8 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
 
 constexpr int kDzRows = 64;
 
-constexpr int64_t kFewRows = 4;  // [1 | 2 | 4 rows, 4096] x [4096, 4096]^T
+// Rows up to which k_rows is used: [1 | 2 | 4,4096]x[4096,4096]^T 5.9, 7.7, 13.6 us; k_gemm takes 8.2 for all three.
+constexpr int64_t kFewRows = 2;
 
 struct FwdSpace {
     void *x, *w;
@@ -246,7 +246,7 @@ dnb_status dnb_connected_act_forward(const void *x, int64_t ldx, const void *w, 
         RowsArgs a{x, w, residual, y, biases, ldx, ldw, ldr, ldy, batch, outputs, inputs, act, dtype};
         a.n = outputs;
         a.k = inputs;
-        if (batch > 4 * 65535) return fail(DNB_ERR_UNSUPPORTED, "%s: too many rows without inputs", what);
+        if (batch > 2 * 65535) return fail(DNB_ERR_UNSUPPORTED, "%s: too many rows without inputs", what);
         const uintptr_t al = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) |
                              (batch > 1 ? (uintptr_t)ldx * 2 : 0) | (outputs > 1 ? (uintptr_t)ldw * 2 : 0);
         return dispatch_dtype16(dtype, [&]<class T>() {

@@ -49,6 +49,7 @@ struct GemmArgs {
     int band;       // output tiles are taken in bands of this many row tiles, down the rows first
     unsigned idesc; // the tensor core's instruction descriptor
     unsigned stage_bytes;  // what a CTA's loads of a stage bring
+    int split;             // CTAs that share a tile (SPLIT)
     const int *m_dev, *k_dev;  // the rows / the reduction's length where the device knows them (NULL: as above)
     unsigned long long wait_ns;
     unsigned *error_word;
@@ -57,23 +58,25 @@ struct GemmArgs {
 constexpr int kGemmThreads = 384;  // 4 warps of roles, 8 of epilogue
 constexpr int kEpilogueWarps = 8;
 constexpr int kBlockK = 64;
+constexpr int kMaxSplit = 4;  // CTAs that may share a tile's k
 constexpr unsigned DEVERR_WAIT_GEMM = 8u;  // a role of a product gave up waiting
 
-template <int CTAS_, int BN_, bool A_MN_, bool B_MN_>
+template <int CTAS_, int BN_, bool A_MN_, bool B_MN_, bool SPLIT_ = false>
 struct GemmCfg {
     static constexpr int CTAS = CTAS_, BN = BN_;
     static constexpr bool A_MN = A_MN_, B_MN = B_MN_;
+    static constexpr bool SPLIT = SPLIT_;      // a cluster of CTAs shares one tile's k
     static constexpr int BM = 128;             // rows of one CTA
     static constexpr int TM = BM * CTAS;       // rows of a tile
     static constexpr int BROWS = BN / CTAS;    // B rows one CTA holds
     static constexpr int A_BYTES = BM * kBlockK * 2, B_BYTES = BROWS * kBlockK * 2;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = STAGE >= 32768 ? 6 : STAGE >= 24576 ? 8 : 10;
+    static constexpr int STAGES = 6;
     static constexpr int TMEM_COLS = 2 * BN;
-    static constexpr int PARTS = BN >= 128 ? 2 : 1;  // epilogue warps that share a row: each EW columns
-    static constexpr int EW = BN / PARTS;
+    static constexpr int EW = BN / 2;          // columns of an epilogue thread: two share a row
     static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 16 * STAGES + 64 + 8 * BN;
-    static_assert(BN % 32 == 0 && (EW == 32 || EW % 64 == 0) && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
+    static_assert(EW % 64 == 0 && BN <= 256 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
+    static_assert(!SPLIT || (CTAS == 1 && BN == 128), "four runs of 32 columns are shared out");
     static_assert(!B_MN || BROWS % 64 == 0, "an MN-major box is 64 wide");
 };
 
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + 8 * b, 1);
-            mbar_init(acc_empty + 8 * b, 4 * C::PARTS * CTAS);
+            mbar_init(acc_empty + 8 * b, kEpilogueWarps * CTAS);
         }
         *gave_up = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -329,8 +332,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     fence_after();
     const uint32_t tmem = *tmem_slot;
     const int m_tiles = g.m_dev ? (*g.m_dev + C::TM - 1) / C::TM : g.m_tiles;
-    const int k_blocks = g.k_dev ? (*g.k_dev + kBlockK - 1) / kBlockK : g.k_blocks;
-    const int tiles = m_tiles * g.n_tiles, step = (int)gridDim.x / CTAS, first = (int)blockIdx.x / CTAS;
+    const int k_all = g.k_dev ? (*g.k_dev + kBlockK - 1) / kBlockK : g.k_blocks;
+    const int tiles = m_tiles * g.n_tiles;
+    // SPLIT: a tile a cluster, this CTA's share of its k blocks; else every step-th tile, all of them
+    const int share = C::SPLIT ? g.split : 1, q = C::SPLIT ? (int)cluster_rank() : 0;
+    const int step = C::SPLIT ? 0x3fffffff : (int)gridDim.x / CTAS, first = (int)blockIdx.x / (C::SPLIT ? share : CTAS);
+    const int kb0 = C::SPLIT ? k_all * q / share : 0, k_blocks = C::SPLIT ? k_all * (q + 1) / share - kb0 : k_all;
 
     if (warp == 0 && lane == 0) {
         // loads
@@ -348,7 +355,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 }
                 const uint32_t a_at = base + s * C::STAGE, b_at = a_at + C::A_BYTES;
                 const uint32_t bar = CTAS == 2 ? map_rank(full + 8 * s, 0) : full + 8 * s;
-                const int k0 = kb * kBlockK;
+                const int k0 = (kb0 + kb) * kBlockK;
                 if (rank == 0) mbar_expect(full + 8 * s, g.stage_bytes * CTAS);
                 if constexpr (C::A_MN) {
 #pragma unroll
@@ -407,62 +414,144 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
             if (issues) commit<CTAS>(acc_full + 8 * b);
         }
-    } else if (warp >= 4) {
-        // epilogue: a warp reads its quarter of the tensor memory's lanes (a lane a row) and half of the columns
-        constexpr int EW = C::EW;
-        const int w = warp & 3, half = (warp - 4) >> 2;
-        float *bias = reinterpret_cast<float *>(tail + 16 * S + 64);  // [2][BN]
-        int n = 0;
-        bool failed = false;
-        for (int t = first; t < tiles; t += step, ++n) {
-            const int b = n & 1;
-            int mt, nt;
-            tile_at(g, m_tiles, t, mt, nt);
-            const int64_t row = (int64_t)mt * C::TM + (int64_t)rank * C::BM + w * 32 + lane,
-                          tile0 = (int64_t)nt * C::BN, col0 = tile0 + half * EW;
-            typename Epi::State st;
-            epi.begin(st, row, col0);
-            typename Epi::Ahead ahead[2];
-            epi.fetch(st, ahead[0], col0);
-            if (epi.bias) {  // the buffer's last readers, two tiles ago, have met at the last tile's barrier
+    }
+
+    // Epilogue: a warp reads its quarter of the tensor memory's lanes (a lane a row) and half of the columns.
+    constexpr int EW = C::EW;
+    const int w = warp & 3, half = (warp - 4) >> 2;
+    float *bias = reinterpret_cast<float *>(tail + 16 * S + 64);  // [2][BN]
+    bool failed = false;
+    // The n-th tile of this CTA.
+    auto take_tile = [&](int t, int n) {
+        const int b = n & 1;
+        int mt, nt;
+        tile_at(g, m_tiles, t, mt, nt);
+        const int64_t row = (int64_t)mt * C::TM + (int64_t)rank * C::BM + w * 32 + lane, tile0 = (int64_t)nt * C::BN,
+                      col0 = tile0 + half * EW;
+        typename Epi::State st;
+        epi.begin(st, row, col0);
+        typename Epi::Ahead ahead[2];
+        epi.fetch(st, ahead[0], col0);
+        if (epi.bias) {  // the buffer's last readers, two tiles ago, have met at the last tile's barrier
+            const int c = threadIdx.x - 128;
+            if (c < C::BN) bias[b * C::BN + c] = tile0 + c < g.n ? epi.bias[tile0 + c] : 0.0f;
+            epilogue_sync();
+        }
+        const float *tile_bias = bias + b * C::BN + half * EW;
+        // a warp that gave up goes on to the barriers, which the other warps may still wait at
+        if (!failed) failed = !__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b, (n >> 1) & 1, g, gave_up));
+        if (failed) return;
+        fence_after();
+        const uint32_t at = tmem + ((uint32_t)(w * 32) << 16) + b * C::BN + half * EW;
+#pragma unroll 1
+        for (int c = 0; c < EW; c += 64) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int64_t col = col0 + c + 32 * h;
+                uint32_t r[32];
+                __syncwarp();  // the loads are the whole warp's
+                if (k_blocks > 0) tmem_load32(at + c + 32 * h, r);
+                if (c + 32 * (h + 1) < EW && col + 32 < g.n) epi.fetch(st, ahead[h ^ 1], col + 32);
+                if (k_blocks > 0) {
+                    tmem_wait(r);
+                } else {  // a sum over nothing
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) r[j] = 0u;
+                }
+                if (c + 32 * (h + 1) >= EW) {  // all read: the next products may overwrite the accumulators
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive_relaxed(CTAS == 2 ? map_rank(acc_empty + 8 * b, 0) : acc_empty + 8 * b);
+                }
+                float2 v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                if (col < g.n) epi.columns(st, v, tile_bias + c + 32 * h, ahead[h], row, col);
+            }
+        }
+        if (col0 < g.n) epi.end(st, row, col0);
+    };
+
+    if constexpr (!C::SPLIT) {
+        if (warp >= 4) {
+            int n = 0;
+            for (int t = first; t < tiles; t += step, ++n) take_tile(t, n);
+        }
+    } else {
+        // The tile's four runs of 32 columns are shared out among the CTAs of the cluster (two or four): each sends its
+        // sums of the other CTAs' columns to them, into shared memory where the stages were (once every CTA's
+        // products have read theirs), and takes its own columns through the epilogue. A column's 128 rows lie
+        // together, so that a warp's lanes write and read 32 neighbours. One CTA taking the whole tile cost 5 us:
+        // 192 KB into one SM.
+        const bool mine = first < tiles && warp >= 4;
+        const int per = 4 / share;                    // runs of a CTA
+        const int own = per == 2 ? 2 * q + half : q;  // this warp's, if it has one
+        const bool takes = mine && (per == 2 || half == (q & 1));
+        float *partial = reinterpret_cast<float *>(tail - S * C::STAGE);  // [share - 1][per][32 columns][128 rows]
+        int mt = 0, nt = 0;
+        if (mine) tile_at(g, m_tiles, first, mt, nt);
+        const int64_t row = (int64_t)mt * C::TM + w * 32 + lane, tile0 = (int64_t)nt * C::BN, col = tile0 + own * 32;
+        typename Epi::State st;
+        typename Epi::Ahead ahead;
+        __syncwarp();
+        if (mine) {
+            epi.begin(st, row, col);
+            if (takes && col < g.n) epi.fetch(st, ahead, col);
+            if (epi.bias) {
                 const int c = threadIdx.x - 128;
-                if (c < C::BN) bias[b * C::BN + c] = tile0 + c < g.n ? epi.bias[tile0 + c] : 0.0f;
+                if (c < C::BN) bias[c] = tile0 + c < g.n ? epi.bias[tile0 + c] : 0.0f;
                 epilogue_sync();
             }
-            const float *tile_bias = bias + b * C::BN + half * EW;
-            // a warp that gave up goes on to the barriers, which the other warps may still wait at
-            if (!failed) failed = !__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b, (n >> 1) & 1, g, gave_up));
-            if (failed || half >= C::PARTS) continue;
+            failed = !__all_sync(0xffffffffu, mbar_wait(acc_full, 0, g, gave_up));
+        }
+        cluster_sync();
+        const uint32_t at = tmem + ((uint32_t)(w * 32) << 16);
+        uint32_t r[32];
+        if (mine && !failed) {
             fence_after();
-            const uint32_t at = tmem + ((uint32_t)(w * 32) << 16) + b * C::BN + half * EW;
+            const bool row_ok = row < (g.m_dev ? (int64_t)*g.m_dev : g.m);
 #pragma unroll 1
-            for (int c = 0; c < EW; c += 64) {
+            for (int i = half; i < 4; i += 2) {
+                const int to = i / per;
+                if (to == q) continue;
+                __syncwarp();
+                if (k_blocks > 0) {
+                    tmem_load32(at + 32 * i, r);
+                    tmem_wait(r);
+                } else {  // a sum over nothing
 #pragma unroll
-                for (int h = 0; h < (EW < 64 ? 1 : 2); ++h) {
-                    const int64_t col = col0 + c + 32 * h;
-                    uint32_t r[32];
-                    __syncwarp();  // the loads are the whole warp's
-                    if (k_blocks > 0) tmem_load32(at + c + 32 * h, r);
-                    if (c + 32 * (h + 1) < EW && col + 32 < g.n) epi.fetch(st, ahead[h ^ 1], col + 32);
-                    if (k_blocks > 0) {
-                        tmem_wait(r);
-                    } else {  // a sum over nothing
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = 0u;
-                    }
-                    if (c + 32 * (h + 1) >= EW) {  // all read: the next products may overwrite the accumulators
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0)
-                            mbar_arrive_relaxed(CTAS == 2 ? map_rank(acc_empty + 8 * b, 0) : acc_empty + 8 * b);
-                    }
-                    float2 v[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                    if (col < g.n) epi.columns(st, v, tile_bias + c + 32 * h, ahead[h], row, col);
+                    for (int j = 0; j < 32; ++j) r[j] = 0u;
                 }
+                const int slot = (q < to ? q : q - 1) * per + (i - to * per);
+                const uint32_t p = map_rank(smem_u32(partial), to) + 4u * (slot * 32 * C::BM + w * 32 + lane);
+                if (row_ok)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(p + 4u * j * C::BM), "r"(r[j]) : "memory");
             }
-            if (col0 < g.n) epi.end(st, row, col0);
+        }
+        __syncwarp();
+        cluster_sync();
+        if (takes && !failed && col < g.n) {
+            if (k_blocks > 0) {
+                tmem_load32(at + 32 * own, r);
+                tmem_wait(r);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] = 0u;
+            }
+            float2 v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+            for (int o = 0; o < share - 1; ++o) {
+                const float *p = partial + ((o * per + own - q * per) * 32 * C::BM + w * 32 + lane);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    v[j] = __fadd2_rn(v[j], make_float2(p[2 * j * C::BM], p[(2 * j + 1) * C::BM]));
+            }
+            epi.columns(st, v, bias + own * 32, ahead, row, col);
+            epi.end(st, row, col);
         }
     }
     __syncwarp();
@@ -473,32 +562,37 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (warp == 2) tmem_free<CTAS>(tmem, C::TMEM_COLS);
 }
 
-// Which tiles a product takes. A CTA's time is its k blocks times what one costs: bound by bringing in the
-// operands (an SM takes about 140 bytes a nanosecond), by the products from 256 columns on. Measured, ns a
-// block: pair 256x256 285, pair 256x128 180, 128x128 240, 128x64 180, 128x32 of few rows 120; then the
-// epilogue of the last tile. The cheapest by waves * blocks wins: few large tiles leave SMs idle, many small
-// ones bring the operands in more often. [1024,4096]x[4096,4096]^T: 128x128 37 us, pair 256x256 23 us;
-// [64,4096]x[4096,4096]^T: 128x128 20 us, 128x32 9 us.
+// Which tiles a product takes: pairs of 256 x 256, single CTAs of 128 x 128, or clusters of 2 or 4 CTAs that share a
+// 128 x 128 tile's k. A block of 64 k costs a pair about 320 ns (its products) and a CTA 175 ns (bringing in the
+// operands and issuing; narrower tiles cost as much), 220 where all SMs bring theirs in for long; handing sums over
+// 1.5 us. The cheapest by waves * blocks wins:
+// few large tiles leave SMs idle, small ones bring the operands in more often. Measured: [1024,4096]x[4096,4096]^T
+// pairs 27 us, single CTAs 37; [4096,8192]x[8192,4096] pairs 187, single CTAs 205; [8 | 64 | 256,4096]x[4096,4096]^T single CTAs 13 to 18 us, clusters 8.2, 9.0, 12.3.
 struct Tiles {
-    int ctas, bn, ew;  // ew: columns of an epilogue thread
+    int ctas, bn, ew, split;  // ew: columns of an epilogue thread
 };
-inline Tiles pick_tiles(int64_t m, int64_t n, int64_t k, bool mn_major) {
-    struct Choice {
-        int ctas, bn, block_ns, tail_ns;
-    };
-    constexpr Choice all[] = {{2, 256, 285, 2500}, {2, 128, 180, 1600}, {1, 128, 240, 1600}, {1, 64, 180, 1400}, {1, 32, 120, 1000}};
+inline Tiles pick_tiles(int64_t m, int64_t n, int64_t k) {
+    constexpr int sms = 148;  // a B200's: workspaces depend on the choice, which must not depend on the current device
     const int64_t blocks = (k + kBlockK - 1) / kBlockK;
-    Tiles best{1, 128, 64};
-    int64_t least = INT64_MAX;
-    for (const Choice &c : all) {
-        if (c.ctas == 2 && m <= 128) continue;                 // half of each pair's rows would be empty
-        if (c.bn == 32 && (mn_major || m > 128)) continue;     // an MN-major box is 64 wide
-        const int64_t tiles = (m + 128 * c.ctas - 1) / (128 * c.ctas) * ((n + c.bn - 1) / c.bn);
-        const int64_t slots = 148 / c.ctas, waves = (tiles + slots - 1) / slots;
-        const int64_t cost = waves * blocks * c.block_ns + c.tail_ns;
+    auto tiles_of = [&](int64_t tm, int64_t tn) { return (m + tm - 1) / tm * ((n + tn - 1) / tn); };
+    auto waves = [](int64_t tiles, int64_t slots) { return (tiles + slots - 1) / slots; };
+    const int64_t singles = tiles_of(128, 128);
+    Tiles best{1, 128, 64, 1};
+    const int64_t single_waves = waves(singles, sms);
+    int64_t least = single_waves * blocks * (single_waves > 1 ? 220 : 175) + 1800;
+    if (m > 128) {  // else half of each pair's rows would be empty
+        const int64_t cost = waves(tiles_of(256, 256), sms / 2) * blocks * 320 + 2500;
         if (cost < least) {
             least = cost;
-            best = {c.ctas, c.bn, c.bn >= 128 ? c.bn / 2 : c.bn};
+            best = {2, 256, 128, 1};
+        }
+    }
+    for (int q = 2; q <= kMaxSplit; q *= 2) {
+        if (singles * q > sms - 12 || blocks < 2 * q) continue;  // one wave: some SMs are left over by the clusters
+        const int64_t cost = (blocks + q - 1) / q * 175 + 1800 + 1500;
+        if (cost < least) {
+            least = cost;
+            best = {1, 128, 32, q};
         }
     }
     return best;
@@ -507,8 +601,8 @@ inline Tiles pick_tiles(int64_t m, int64_t n, int64_t k, bool mn_major) {
 // Launches the product of a and b (already TMA-ready). With m_dev / k_dev, m and k are what they may reach.
 template <class C, class Epi>
 dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k, const Epi &epi,
-                       const DeviceState *ds, cudaStream_t s, const char *what, const int *m_dev = nullptr,
-                       const int *k_dev = nullptr) {
+                       const DeviceState *ds, cudaStream_t s, const char *what, int split = 1,
+                       const int *m_dev = nullptr, const int *k_dev = nullptr) {
     static std::atomic<int> opted[kMaxDevices];
     auto kernel = k_gemm<C, Epi>;
     if (!opted[ds->device].load(std::memory_order_acquire)) {
@@ -533,6 +627,7 @@ dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m,
     g.n_tiles = (int)nt;
     g.k_blocks = (int)((k + kBlockK - 1) / kBlockK);
     g.band = 8;
+    g.split = split;
     g.stage_bytes = (unsigned)(a_rows * kBlockK * 2 + C::B_BYTES);
     g.m_dev = m_dev;
     g.k_dev = k_dev;
@@ -544,16 +639,17 @@ dnb_status launch_gemm(const Operand &a, const Operand &b, int dtype, int64_t m,
     g.error_word = ds->error_word;
     const int64_t slots = ds->sm_count / C::CTAS, tiles = mt * nt;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((tiles < slots ? tiles : slots) * C::CTAS));
+    const int cluster = C::SPLIT ? split : C::CTAS;
+    cfg.gridDim = dim3((unsigned)(C::SPLIT ? tiles * split : (tiles < slots ? tiles : slots) * C::CTAS));
     cfg.blockDim = dim3(kGemmThreads);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = C::CTAS;
+    at[0].val.clusterDim.x = (unsigned)cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = C::CTAS > 1 ? 1 : 0;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
     DNB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, g, epi));
     return after_launch(s, what);
 }

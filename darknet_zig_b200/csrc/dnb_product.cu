@@ -7,17 +7,12 @@ namespace {
 template <bool A_MN, bool B_MN>
 dnb_status run(const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k, const EpiOut &e,
                const DeviceState *ds, cudaStream_t s, const char *what, const int *m_dev, const int *k_dev) {
-    const Tiles t = pick_tiles(m, n, k, B_MN);
-    if (t.ctas == 2 && t.bn == 256)
-        return launch_gemm<GemmCfg<2, 256, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
+    const Tiles t = pick_tiles(m, n, k);
     if (t.ctas == 2)
-        return launch_gemm<GemmCfg<2, 128, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
-    if constexpr (!A_MN && !B_MN)
-        if (t.bn == 32)
-            return launch_gemm<GemmCfg<1, 32, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
-    if (t.bn == 64)
-        return launch_gemm<GemmCfg<1, 64, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
-    return launch_gemm<GemmCfg<1, 128, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev, k_dev);
+        return launch_gemm<GemmCfg<2, 256, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, 1, m_dev, k_dev);
+    if (t.split > 1)
+        return launch_gemm<GemmCfg<1, 128, A_MN, B_MN, true>>(a, b, dtype, m, n, k, e, ds, s, what, t.split, m_dev, k_dev);
+    return launch_gemm<GemmCfg<1, 128, A_MN, B_MN>>(a, b, dtype, m, n, k, e, ds, s, what, 1, m_dev, k_dev);
 }
 
 }  // namespace

@@ -335,18 +335,14 @@ __global__ void __launch_bounds__(256) k_delta_sums(const float *sums, const int
     }
 }
 
-// The tiles of the two products whose results stay in the epilogue: those of pick_tiles, in three of its shapes.
-Tiles xent_tiles(int64_t m, int64_t n, int64_t k) {
-    Tiles t = pick_tiles(m, n, k, true);
-    if (t.ctas == 2 && t.bn == 128) t = {1, 128, 64};
-    return t;
-}
+// The products whose results stay in the epilogue.
 template <class Epi>
 dnb_status xent_product(const Tiles &t, const Operand &a, const Operand &b, int dtype, int64_t m, int64_t n, int64_t k,
                         const Epi &e, const DeviceState *ds, cudaStream_t s, const char *what, const int *m_dev) {
-    if (t.ctas == 2) return launch_gemm<GemmCfg<2, 256, false, false>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev);
-    if (t.bn == 64) return launch_gemm<GemmCfg<1, 64, false, false>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev);
-    return launch_gemm<GemmCfg<1, 128, false, false>>(a, b, dtype, m, n, k, e, ds, s, what, m_dev);
+    if (t.ctas == 2) return launch_gemm<GemmCfg<2, 256, false, false>>(a, b, dtype, m, n, k, e, ds, s, what, 1, m_dev);
+    if (t.split > 1)
+        return launch_gemm<GemmCfg<1, 128, false, false, true>>(a, b, dtype, m, n, k, e, ds, s, what, t.split, m_dev);
+    return launch_gemm<GemmCfg<1, 128, false, false>>(a, b, dtype, m, n, k, e, ds, s, what, 1, m_dev);
 }
 
 // ---- the caller's workspace ----
@@ -366,7 +362,7 @@ struct FwdSpace {
 FwdSpace fwd_space(void *ws, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t m, int64_t k, int64_t n) {
     Carver c(ws);
     FwdSpace f{};
-    f.shape = xent_tiles(m, n, k);
+    f.shape = pick_tiles(m, n, k);
     f.tiles = (n + f.shape.ew - 1) / f.shape.ew;
     f.part = static_cast<float2 *>(c.take(f.tiles * m * 8));
     f.at_label = static_cast<float *>(c.take(m * 4));
@@ -572,7 +568,7 @@ dnb_status dnb_connected_xent_backward(const void *x, int64_t ldx, const void *w
         e.sums = bias_updates ? f.sums : nullptr;
         e.scale = scale;
         e.dtype = dtype;
-        DNB_TRY(xent_product(xent_tiles(batch, n, inputs), xp, wq, dtype, rows, n, inputs, e, ds, s, what, f.count));
+        DNB_TRY(xent_product(pick_tiles(batch, n, inputs), xp, wq, dtype, rows, n, inputs, e, ds, s, what, f.count));
         if (bias_updates) {
             k_delta_sums<<<(unsigned)((n + 31) / 32), 256, 0, s>>>(f.sums, f.count, n, f.piece, bias_updates + c0, add_w);
             DNB_TRY(after_launch(s, what));

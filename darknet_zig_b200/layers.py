@@ -94,6 +94,77 @@ class BatchNorm:
         return delta
 
 
+class GroupNorm:
+    """Group norm + activation on a channels-last tensor [batch, spatial, filters] (f32, bf16 or f16): the
+    batchnorm layer's place where the statistics may not depend on the batch. Keeps the forward's input (and
+    output, where the activation's gradient needs its sign) for the backward."""
+
+    def __init__(self, batch: int, spatial: int, filters: int, groups: int, activation: int = gpu.LEAKY,
+                 eps: float = 1e-5, device="cuda"):
+        self.batch, self.spatial, self.filters, self.groups = batch, spatial, filters, groups
+        self.activation, self.eps = activation, eps
+        self.scales = torch.ones(filters, dtype=torch.float32, device=device)
+        self.biases, self.scale_updates, self.bias_updates = (
+            torch.zeros(filters, dtype=torch.float32, device=device) for _ in range(3))
+        self.mean = torch.empty(batch, groups, dtype=torch.float32, device=device)
+        self.rstd = torch.empty_like(self.mean)
+        self.x = self.output = None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        self.x, self.output = x, torch.empty_like(x)
+        gpu.gnActForward(x, self.output, self.batch, self.spatial, self.filters, self.groups, self.scales, self.biases,
+                         self.eps, self.mean, self.rstd, self.activation)
+        return self.output
+
+    def backward(self, delta: torch.Tensor) -> torch.Tensor:
+        """delta: of the output; overwritten with the input's, and returned. The updates are added to."""
+        smooth = self.activation in (gpu.LINEAR, gpu.LOGISTIC)
+        gpu.gnActBackward(self.x, None if smooth else self.output, delta, delta, self.batch, self.spatial, self.filters,
+                          self.groups, self.scales, self.biases, self.mean, self.rstd, self.bias_updates,
+                          self.scale_updates, self.activation)
+        return delta
+
+
+class Connected:
+    """The connected layer (connected.zig) on 16-bit tensors, which on channels-last rows is the 1x1 convolution:
+    fp32 master weights and updates, their 16-bit copy for the products, an optional residual before the
+    activation (the shortcut layer's place)."""
+
+    def __init__(self, batch: int, inputs: int, outputs: int, activation: int = gpu.LEAKY, dtype=torch.bfloat16,
+                 device="cuda"):
+        self.batch, self.inputs, self.outputs, self.activation = batch, inputs, outputs, activation
+        self.weights = (torch.rand(outputs, inputs, device=device) * 2 - 1) * (2.0 / inputs) ** 0.5
+        self.weights16 = self.weights.to(dtype)
+        self.weight_updates = torch.zeros_like(self.weights)
+        self.biases = torch.zeros(outputs, device=device)
+        self.bias_updates = torch.zeros_like(self.biases)
+        self.x = self.output = None
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        self.x = x
+        self.output = torch.empty(self.batch, self.outputs, device=x.device, dtype=x.dtype)
+        gpu.connectedActForward(x, self.weights16, self.biases, residual, self.output, self.batch, self.inputs,
+                                self.outputs, self.activation)
+        return self.output
+
+    def backward(self, delta: torch.Tensor, need_input: bool = True) -> torch.Tensor | None:
+        """delta: of the output; overwritten with the residual's (delta through the activation). Returns the
+        input's (None unless needed). The updates are added to."""
+        dx = torch.empty(self.batch, self.inputs, device=delta.device, dtype=delta.dtype) if need_input else None
+        linear = self.activation == gpu.LINEAR
+        gpu.connectedActBackward(self.x, self.weights16, None if linear else self.output, delta,
+                                 None if linear else delta, dx, self.bias_updates, self.weight_updates, self.batch,
+                                 self.inputs, self.outputs, self.activation)
+        return dx
+
+    def update(self, learning_rate: float, momentum: float, decay: float, batch: int) -> None:
+        """connected.updateGpu: biases as sgd_update; the weights in one pass that leaves their 16-bit copy."""
+        gpu.axpy(self.outputs, learning_rate / batch, self.bias_updates, self.biases)
+        gpu.scal(self.outputs, momentum, self.bias_updates)
+        gpu.sgdMomentumMixed(self.weights, self.weight_updates, None, self.weights16, self.outputs, self.inputs,
+                             learning_rate, momentum, decay, batch)
+
+
 def sgd_update(weights, weight_updates, biases, bias_updates, scales, scale_updates, learning_rate: float,
                momentum: float, decay: float, batch: int, fused: bool = True) -> None:
     """convolutional.updateGpu (convolutional.zig:311-335), SGD branch."""
