@@ -400,7 +400,9 @@ dnb_status dnb_syncbn_backward_apply(const float *x, const float *y, const float
 /*   - an output may not overlap an input or another output, except where its entry says    */
 /*     that it may be the same tensor (same pointer and ld);                               */
 /*   - results do not depend on timing: the same call gives the same bits on the same GPU   */
-/*     model.                                                                              */
+/*     model;                                                                              */
+/*   - sizes beyond the kernels' limits (2^31 - 1 rows or columns of a product, 4 million      */
+/*     rows of a backward) return DNB_ERR_UNSUPPORTED.                                       */
 /* ------------------------------------------------------------------------------------ */
 
 /* element types */
