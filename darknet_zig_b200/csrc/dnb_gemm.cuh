@@ -10,8 +10,13 @@
 // 128*CTAS x BN at a time. Warp 0 issues the loads into a ring of stages (64 k each), warp 1 of the pair's
 // first CTA issues the products into one of two accumulators in tensor memory, warps 4-11 take the other
 // accumulator through the epilogue meanwhile (two warps a scheduler, each half of the columns: one alone
-// leaves its latencies bare and took 7 us for a tile that two finish in 3). A pair halves the operand traffic per SM: each CTA holds its
-// own 128 rows of A and half of B's rows, and the products read both CTAs' shared memory.
+// leaves its latencies bare and took 7 us for a tile that two finish in 3). A pair halves the operand traffic per
+// SM: each CTA holds its own 128 rows of A and half of B's rows, and the products read both CTAs' shared memory.
+// Where tiles are few, a cluster of CTAs shares a tile's k (SPLIT).
+//
+// Bound by the tensor cores from some 256 rows and columns a side on: [2048,4096]x[4096,4096]^T bf16 48 us, 1430
+// TFLOP/s; [8192,16384]x[4096,16384]^T with residual 730 us (1506) in a single launch, 850 us (1290) back to back
+// under the power cap.
 //
 // Every wait is bounded (dnb_set_wait_limit_ms): a role whose wait gives up sets the error word and
 // leaves its loop; the others' waits then end the same way, the CTA (pair) meets at its last barrier and

@@ -9,7 +9,8 @@
 // elements, so s's own distance from the mean is among the deviations that make up the variance, and no mean,
 // however far from 0, cancels. Each thread's (count, mean, squared deviations) are merged as Chan, Golub and LeVeque
 // do, about one of the means, in a fixed order. With a second walk over shared memory for the deviations instead,
-// [128,784,256] bf16 took 45 us, bound by instructions (30 an element).
+// [128,784,256] bf16 took 45 us, bound by instructions (30 an element); so it takes 23 us (16 an element; 103 MB at
+// 4.5 TB/s).
 #include "dnb_gn.cuh"
 
 namespace dnb {

@@ -3,9 +3,10 @@
 //
 // A unit is one image's run of whole groups, `cb` channels wide (64 bytes of a row or more, so that the
 // accesses of a row fill their sectors) and all `spatial` rows tall. A CTA, or a cluster of up to 8 CTAs
-// that split the rows, loads a unit into shared memory once, forms the statistics there and writes the
-// outputs from there, so every tensor crosses HBM once. Units beyond what 8 CTAs can hold take the
-// streaming path: partial statistics of row chunks, a merge, and a second read of the inputs.
+// that split the rows, takes a unit: the forward loads it into shared memory once, forms the statistics there
+// and writes the outputs from there; the backward walks it twice, the second time in the L2 cache. So every
+// tensor crosses HBM once. Units beyond what 8 CTAs can hold (or the cache keep) take the streaming path:
+// partial statistics of row chunks, a merge, and a second read of the inputs.
 //
 // A thread owns one vector of channels (VB bytes) and every RL-th row, so per-channel values sit in its
 // registers: V = cb / N vectors make a row; RL = T / V threads share a column, or, where a row is longer
