@@ -81,13 +81,27 @@ struct EpiOut {
             for (int i = 0; i < 4; ++i) v[4 * j + i] = __fadd2_rn(v[4 * j + i], f[i]);
         }
     }
+    // The first n elements of a vector at the row's end.
     template <class T>
-    __device__ __forceinline__ void load_add(float2 (&v)[16], int64_t row, int64_t col) const {
+    static __device__ __forceinline__ uint4 some(const T *p, int n) {
+        typename Vec<T, 16>::U u;
+        u.raw = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < Vec<T, 16>::N; ++i)
+            if (i < n) u.e[i] = p[i];
+        return u.raw;
+    }
+    template <class T>
+    __device__ __forceinline__ void load_add(float2 (&v)[16], int64_t row, int64_t col, int cols) const {
         const T *p = static_cast<const T *>(add) + row * ld_add + col;
         constexpr int N = 16 / (int)sizeof(T);
         uint4 raw[32 / N];
 #pragma unroll
-        for (int j = 0; j < 32 / N; ++j) raw[j] = reinterpret_cast<const uint4 *>(p)[j];
+        for (int j = 0; j < 32 / N; ++j) {
+            raw[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (j * N + N <= cols) raw[j] = reinterpret_cast<const uint4 *>(p)[j];
+            else if (j * N < cols) raw[j] = some(p + j * N, cols - j * N);
+        }
 #pragma unroll
         for (int j = 0; j < 32 / N; ++j) {
             float2 f[N / 2];
@@ -97,7 +111,7 @@ struct EpiOut {
         }
     }
     template <class T>
-    __device__ __forceinline__ void store(const float2 (&v)[16], int64_t row, int64_t col) const {
+    __device__ __forceinline__ void store(const float2 (&v)[16], int64_t row, int64_t col, int cols) const {
         T *p = static_cast<T *>(out) + row * ld + col;
         constexpr int N = 16 / (int)sizeof(T);
         uint4 raw[32 / N];
@@ -108,12 +122,22 @@ struct EpiOut {
             for (int i = 0; i < N / 2; ++i) f[i] = v[j * N / 2 + i];
             raw[j] = Pairs<T, 16>::pack(f);
         }
-        if (wide_out) {
+        if (wide_out && cols == 32) {
 #pragma unroll
             for (int j = 0; j < 32 / N; j += 2) store32(reinterpret_cast<uint4 *>(p) + j, raw[j], raw[j + 1]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 32 / N; ++j) reinterpret_cast<uint4 *>(p)[j] = raw[j];
+            for (int j = 0; j < 32 / N; ++j) {
+                if (j * N + N <= cols) {
+                    reinterpret_cast<uint4 *>(p)[j] = raw[j];
+                } else if (j * N < cols) {
+                    typename Vec<T, 16>::U u;
+                    u.raw = raw[j];
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (j * N + i < cols) p[j * N + i] = u.e[i];
+                }
+            }
         }
     }
     __device__ __forceinline__ void activate(float2 (&v)[16]) const {
@@ -125,17 +149,30 @@ struct EpiOut {
         default: activate_any(v, act);
         }
     }
-    __device__ __forceinline__ float load_one(int64_t at) const {
-        if (add_type == DNB_F32) return static_cast<const float *>(add)[at];
-        if (add_type == DNB_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(add)[at]);
-        return __half2float(static_cast<const __half *>(add)[at]);
+    // The addend's elements of a column in the warp's 32 rows (row: lane i's is row i's index, or -1): all on their way
+    // before the first is needed.
+    template <class T>
+    __device__ __forceinline__ void add_rows(float (&u)[32], int64_t row, int64_t col, bool in) const {
+        const T *p = static_cast<const T *>(add) + col;
+        T got[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int64_t at = __shfl_sync(0xffffffffu, row, i);
+            got[i] = in && at >= 0 ? p[at * ld_add] : Elem<T>::from(0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) u[i] += Elem<T>::to(got[i]);
     }
-    __device__ __forceinline__ void store_one(int64_t at, float v) const {
-        if (out_type == DNB_F32) static_cast<float *>(out)[at] = v;
-        else if (out_type == DNB_BF16) static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(v);
-        else static_cast<__half *>(out)[at] = __float2half_rn(v);
+    template <class T>
+    __device__ __forceinline__ void store_rows(const float2 (&v)[16], int64_t row, int64_t col, bool in) const {
+        T *p = static_cast<T *>(out) + col;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int64_t at = __shfl_sync(0xffffffffu, row, i);
+            if (in && at >= 0) p[at * ld] = Elem<T>::from(i & 1 ? v[i / 2].y : v[i / 2].x);
+        }
     }
-    // Rows off the 16-byte boundaries, or the ragged edge: the warp turns its 32 x 32 values over, so that its lanes
+    // Rows off the 16-byte boundaries: the warp turns its 32 x 32 values over, so that its lanes
     // hold neighbouring columns of a row, and reads and writes a row at a time. (A lane's own row element by element
     // touches 32 sectors an access: 157 us against 85 at a backward of [900,8183]x[316,8183].)
     __device__ __forceinline__ void ragged(int64_t row, float2 (&v)[16], int64_t col, int cols) const {
@@ -160,25 +197,21 @@ struct EpiOut {
         // u[i]: row i of the warp's, column `lane`
         const bool in = lane < cols;
         if (add) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int64_t to = __shfl_sync(0xffffffffu, row, i);
-                if (in && to >= 0) u[i] += load_one(to * ld_add + col + lane);
-            }
+            if (add_type == DNB_F32) add_rows<float>(u, row, col + lane, in);
+            else if (add_type == DNB_BF16) add_rows<__nv_bfloat16>(u, row, col + lane, in);
+            else add_rows<__half>(u, row, col + lane, in);
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = make_float2(u[2 * j], u[2 * j + 1]);
         activate(v);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int64_t to = __shfl_sync(0xffffffffu, row, i);
-            if (in && to >= 0) store_one(to * ld + col + lane, i & 1 ? v[i / 2].y : v[i / 2].x);
-        }
+        if (out_type == DNB_F32) store_rows<float>(v, row, col + lane, in);
+        else if (out_type == DNB_BF16) store_rows<__nv_bfloat16>(v, row, col + lane, in);
+        else store_rows<__half>(v, row, col + lane, in);
     }
     __device__ __forceinline__ void columns(State &s, float2 (&v)[16], const float *tile_bias, const Ahead &h, int64_t,
                                             int64_t col) const {
         const int cols = (int)(n - col < 32 ? n - col : 32);
-        const bool whole = vec_out && cols == 32 && (!add || vec_add);  // the same in every lane
+        const bool whole = vec_out && (!add || vec_add);  // the same in every lane
         if (whole && s.row < 0) return;
         const int64_t row = s.row;
         if (s.f != 1.0f) {
@@ -191,17 +224,17 @@ struct EpiOut {
             return;
         }
         if (add) {
-            if (early) {
+            if (early && cols == 32) {
                 if (add_type == DNB_BF16) add_fetched<__nv_bfloat16>(v, h);
                 else add_fetched<__half>(v, h);
-            } else if (add_type == DNB_F32) load_add<float>(v, row, col);
-            else if (add_type == DNB_BF16) load_add<__nv_bfloat16>(v, row, col);
-            else load_add<__half>(v, row, col);
+            } else if (add_type == DNB_F32) load_add<float>(v, row, col, cols);
+            else if (add_type == DNB_BF16) load_add<__nv_bfloat16>(v, row, col, cols);
+            else load_add<__half>(v, row, col, cols);
         }
         activate(v);
-        if (out_type == DNB_F32) store<float>(v, row, col);
-        else if (out_type == DNB_BF16) store<__nv_bfloat16>(v, row, col);
-        else store<__half>(v, row, col);
+        if (out_type == DNB_F32) store<float>(v, row, col, cols);
+        else if (out_type == DNB_BF16) store<__nv_bfloat16>(v, row, col, cols);
+        else store<__half>(v, row, col, cols);
     }
     static __device__ __noinline__ float activate_one(float v, int a) { return act_fwd_any(v, a); }
     static __device__ __forceinline__ void activate_any(float2 (&v)[16], int a) {
